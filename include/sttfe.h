@@ -293,6 +293,90 @@ int sttfe_pitch_shift_plan(const int32_t* lengths, const int32_t* n_steps, int b
 int sttfe_pitch_shift(float* pcm, const int64_t* offsets, const int32_t* lengths, int batch, const int64_t* layout,
                       const int64_t* dev_layout, int mode, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------- token objectives --------------
+ * What a model answers with, against the labels the collator pads with -100 (src/data.py:500): label log probabilities
+ * with entropy and top alternatives, and distillation from a teacher's top logits.  The reference has neither; its models
+ * compute their cross entropy inside HF's forward (src/models.py, train.py:300-309).
+ *
+ * Common arguments
+ *   logits       : device, STTFE_DTYPE_*; row r of outer * inner rows is (r / inner, r % inner) and starts at element
+ *                  (r / inner) * stride_outer + (r % inner) * stride_inner; its vocab elements are contiguous.  Strides are
+ *                  >= 0, count elements, and may be anything else (a slice of positions, an expanded batch).  Rows need the
+ *                  alignment of one element only.  At most STTFE_MAX_ROWS rows, vocab in [1, STTFE_MAX_VOCAB].
+ *   labels       : device int64 [outer * inner]; rows with label == ignore_index hold no token: they are not read, their
+ *                  results are 0 (ids -1, top log probabilities -inf) and their gradient is 0.  Any other label outside
+ *                  [0, vocab) cannot be reported without synchronising: the row's results and its gradient are NaN.
+ *   temperature  : > 0; the softmax is that of logits / temperature.
+ *   stats        : device float32 [outer * inner][4], written by the forward call for the gradient call (NULL: not wanted).
+ * A row that holds NaN or +inf, or nothing but -inf, has no softmax: its results are NaN, as torch.log_softmax's are
+ * (alternatives: NaN counts as the largest value).  A -inf logit among others has probability 0 and adds nothing.
+ * All sums are float32 or wider and in a fixed order: the same inputs give the same bits.
+ */
+#define STTFE_DTYPE_F32 0
+#define STTFE_DTYPE_F16 1
+#define STTFE_DTYPE_BF16 2
+#define STTFE_MAX_TOP 64                 /* alternatives per row */
+#define STTFE_MAX_ROWS 16777216
+#define STTFE_MAX_VOCAB 4194304
+#define STTFE_REDUCE_NONE 0
+#define STTFE_REDUCE_SUM 1
+#define STTFE_REDUCE_MEAN 2
+
+/* Bytes of device workspace of sttfe_token_logprobs (0: NULL will do). */
+int sttfe_token_logprobs_workspace_bytes(int64_t rows, int vocab, int dtype, int top_k, size_t* bytes);
+
+/*
+ * labels       : NULL = every row counts (then logprobs must be NULL).
+ * logprobs     : device float32 [rows] or NULL: log probability of the label.
+ * entropy      : device float32 [rows] or NULL: entropy of the row in nats.
+ * top_ids / top_logprobs : device int64 / float32 [rows][top_k]: the top_k largest logits, largest first, equal ones in the
+ *                order of their index; top_k in [0, min(vocab, STTFE_MAX_TOP)].
+ */
+int sttfe_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                         int64_t stride_inner, int vocab, const int64_t* labels, int64_t ignore_index, float temperature,
+                         int top_k, float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* grad (device, dtype of the logits, [rows][vocab] contiguous) from the upstream gradients of the three outputs (each device
+ * float32 or NULL: none); top_ids as the forward call wrote them.  Rounded to the logits' type once. */
+int sttfe_token_logprobs_grad(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                              int64_t stride_inner, int vocab, const int64_t* labels, int64_t ignore_index, float temperature,
+                              const float* stats, const float* g_logprobs, const float* g_entropy, int top_k,
+                              const int64_t* top_ids, const float* g_top, void* grad, void* stream);
+
+/* Bytes of device workspace of sttfe_distill_loss (0: NULL will do). */
+int sttfe_distill_workspace_bytes(int64_t rows, int vocab, int dtype, size_t* bytes);
+
+/*
+ * loss_r = alpha * temperature^2 * sum_k q_k (log q_k - log p^t_{id_k}) + (1 - alpha) * (-log p_label), with
+ * q = softmax(teacher_logits / temperature) over the row's kept entries, p^t = softmax(logits / temperature),
+ * p = softmax(logits).
+ * teacher_ids / teacher_logits : device int64 / float32 [rows][teacher_k], teacher_k in [1, STTFE_MAX_TOP]; entries with a
+ *                negative id are not kept, a row without any (or with only -inf logits) has no teacher term; the same id
+ *                twice counts with both weights; an id >= vocab makes the row's loss and gradient NaN.
+ * reduction    : NONE: losses only.  SUM / MEAN: factor[0] = weight (SUM) or weight / (number of rows whose label is not
+ *                ignore_index; 1 if there is none) (MEAN), total[0] = factor[0] * (sum of the losses); device float32.
+ * losses       : device float32 [rows], without the weight.
+ * grad         : NULL, or device [rows][vocab] contiguous, dtype of the logits: d(total[0]) / d(logits) (reduction NONE:
+ *                of the sum of the losses), rounded once.
+ */
+int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                       int64_t stride_inner, int vocab, const int64_t* labels, int64_t ignore_index,
+                       const int64_t* teacher_ids, const float* teacher_logits, int teacher_k, float temperature,
+                       float alpha, float weight, int reduction, float* losses, float* total, float* factor,
+                       float* stats, void* grad, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradient alone, from the forward call's stats: row r's is multiplied by factor[0] * g[0] * g_rows[r] (device float32,
+ * each or NULL = 1; factor as the forward call wrote it). */
+int sttfe_distill_grad(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t stride_outer,
+                       int64_t stride_inner, int vocab, const int64_t* labels, int64_t ignore_index,
+                       const int64_t* teacher_ids, const float* teacher_logits, int teacher_k, float temperature,
+                       float alpha, const float* stats, const float* factor, const float* g, const float* g_rows,
+                       void* grad, void* stream);
+
+/* grad *= g[0] in place (count elements); reads and writes nothing if g[0] is 1. */
+int sttfe_distill_rescale(void* grad, int dtype, int64_t count, const float* g, void* stream);
+
 /* Consecutive 48-frame tiles per work item of the STFT kernels (0 = automatic, the default: the kernel derives it
  * from the clip lengths it finds on the device -- general kernel: a third of the clip for uniform batches, about eight
  * items per workgroup otherwise, within [3, 21]; 12-wave kernel: about eight (uniform) or sixteen (ragged) items per
@@ -314,7 +398,8 @@ int sttfe_set_whisper_uniform_kernel(int on);
  * sttfe_timing_enable(capacity) allocates `capacity` event pairs (0 disables and frees them);
  * sttfe_timing_query(name, ...) returns the summed duration and launch count of one kernel
  * ("whisper_stft_mel", "whisper_clamp_fill", "kaldi_fbank", "kaldi_cmvn", "resample_peak",
- * "normalize_trim", "waveform_augment", "pitch_shift", "whisper_stft_mel12" -- the 12-wave STFT kernel of uniform
+ * "normalize_trim", "waveform_augment", "pitch_shift", "token_logprobs", "token_logprobs_grad", "distill_loss",
+ * "distill_grad", "whisper_stft_mel12" -- the 12-wave STFT kernel of uniform
  * batches, launched beside "whisper_stft_mel" by the calls that qualify for it: the one the batch is not for returns at
  * once) since the last enable/reset; it synchronises on the recorded events.
  */

@@ -10,6 +10,7 @@ from .augment import GpuWaveformAugmenter, SpecAugmentSampler, WaveformAugmentSa
 from .config import AugmentationConfig, DataConfig  # noqa: F401
 from .data import AudioCollator, GpuFrontEnd  # noqa: F401
 from .feature_cache import FeatureCacheDataset, FeatureCacheWriter  # noqa: F401
+from .objectives import TokenScores, distillation_loss, distillation_loss_and_grad, token_logprobs  # noqa: F401
 from .preprocess import GpuAudioPreprocessor, PackedAudio, PinnedIngestRing, ResamplePlan  # noqa: F401
 from .processors import (BatchFeature, HipSpeech2TextFeatureExtractor, HipWhisperFeatureExtractor,  # noqa: F401
                          TorchWhisperFeatureExtractor, pack_clips)

@@ -27,6 +27,7 @@ def _declare(lib):
     lib.sttfe_strerror.restype = c_char_p
     lib.sttfe_strerror.argtypes = [c_int]
     lib.sttfe_last_error_detail.restype = c_char_p
+    rows = [p, c_int, c_int64, c_int64, c_int64, c_int64, c_int]      # logits, dtype, outer, inner, 2 strides, vocab
     sigs = {
         "sttfe_whisper_tables_bytes": [c_int, POINTER(c_size_t)],
         "sttfe_whisper_tables_build": [c_int, p, c_size_t],
@@ -60,6 +61,13 @@ def _declare(lib):
         "sttfe_waveform_augment": [p, p, p, c_int, c_int64, p, p, p, c_int, p],
         "sttfe_pitch_shift_plan": [p, p, c_int, c_int, c_int, p, p],
         "sttfe_pitch_shift": [p, p, p, c_int, p, p, c_int, p, c_size_t, p],
+        "sttfe_token_logprobs_workspace_bytes": [c_int64, c_int, c_int, c_int, POINTER(c_size_t)],
+        "sttfe_token_logprobs": rows + [p, c_int64, c_float, c_int, p, p, p, p, p, p, c_size_t, p],
+        "sttfe_token_logprobs_grad": rows + [p, c_int64, c_float, p, p, p, c_int, p, p, p, p],
+        "sttfe_distill_workspace_bytes": [c_int64, c_int, c_int, POINTER(c_size_t)],
+        "sttfe_distill_loss": rows + [p, c_int64, p, p, c_int, c_float, c_float, c_float, c_int, p, p, p, p, p, p, c_size_t, p],
+        "sttfe_distill_grad": rows + [p, c_int64, p, p, c_int, c_float, c_float, p, p, p, p, p, p],
+        "sttfe_distill_rescale": [p, c_int, c_int64, p, p],
     }
     for name, args in sigs.items():
         fn = getattr(lib, name, None)

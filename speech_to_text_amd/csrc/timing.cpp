@@ -25,7 +25,8 @@ int g_stride = 1;
 unsigned g_seen[kTimedKernelCount] = {};
 const char* const kNames[kTimedKernelCount] = {"whisper_stft_mel", "whisper_clamp_fill", "kaldi_fbank",
                                                "kaldi_cmvn", "resample_peak", "normalize_trim", "waveform_augment", "pitch_shift",
-                                               "whisper_stft_mel12"};
+                                               "whisper_stft_mel12", "token_logprobs", "token_logprobs_grad", "distill_loss",
+                                               "distill_grad"};
 }  // namespace
 
 bool timing_enabled() { return g_enabled; }

@@ -74,6 +74,8 @@ class AudioCollator:
                       "text": [s.get("text", "") for s in batch]}
             if attention_mask is not None:
                 result["attention_mask"] = attention_mask
+            if any("teacher_ids" in s for s in batch):
+                result.update(self._teacher(batch, labels.shape[1]))
             return result
         elif self.device == "cuda":
             # src/data.py:519-527, plus "audio_lengths": zero padding hides where a clip ends, and the
@@ -85,6 +87,21 @@ class AudioCollator:
                     "audio_lengths": torch.tensor([c.shape[0] for c in clips], dtype=torch.int32)}
         else:
             raise ValueError(f"Unsupported processing device: {self.device}. Must be 'cpu' or 'cuda'.")
+
+
+    @staticmethod
+    def _teacher(batch, positions: int) -> Dict[str, torch.Tensor]:
+        """A teacher's kept alternatives (``FeatureCacheDataset``) beside the labels, as ``distillation_loss`` takes them:
+        (B, positions, K), padded with id -1 / logit -inf (positions behind a clip's labels, clips without a teacher)."""
+        top = max(int(s["teacher_ids"].shape[1]) for s in batch if "teacher_ids" in s)
+        ids = torch.full((len(batch), positions, top), -1, dtype=torch.int64)
+        logits = torch.full((len(batch), positions, top), float("-inf"))
+        for b, s in enumerate(batch):
+            if "teacher_ids" in s:
+                t = torch.as_tensor(s["teacher_ids"])
+                ids[b, :t.shape[0], :t.shape[1]] = t
+                logits[b, :t.shape[0], :t.shape[1]] = torch.as_tensor(s["teacher_logits"])
+        return {"teacher_ids": ids, "teacher_logits": logits}
 
 
 class GpuFrontEnd:

@@ -1,0 +1,530 @@
+"""Token scoring and distillation on the GPU against oracle/objectives.py (float64, from the formulas).
+
+Bars, with u = 2^-24 (half a step of float32), lp in nats, n_add = the longest chain of float32 additions behind a sum:
+  * S = sum 2^y carries n_add u from adding, and per term 2 |y| u ln 2 (y = c (z - m) is rounded, c too) + 2 u (exp2); what a term
+    with a large |y| adds is weighted by 2^y, so the mean of |y| over the terms is at most log2 V < 22:  |dS / S| <= (n_add + 48) u.
+  * lp = (y - log2 S) ln 2:  |d| <= (n_add + 48 + 22 + 4 |lp|) u   (the rounding of log2 S <= log2 V is 22 u)
+  * H = (log2 S - W / S) ln 2, |W / S| <= log2 V:  |d| <= (n_add + 70) (1 + log2 V) u
+  * gradient: each term carries the relative error of its p, (n_add + 70 + 4 |lp|) u, and the sum is rounded to the type once:
+    |d| <= (n_add + 80 + 4 |lp|) u * (sum of the terms' sizes) + eps_type / 2 |grad| + half the type's smallest step.
+    4 |lp| p u is largest at p = 1/e and below 2 u.
+  * loss: alpha tau^2 sum q (log q - lp): q has relative error (64 + 70 + ...) u, so each factor's error is bounded by
+    (n_add + 160 + 4 (|lp| + |log q|)) u times alpha tau^2 q, plus the label's (1 - alpha) lp.
+n_add: no kernel adds more than V / 256 terms in a row before it joins 256 or more partial sums in a tree (<= 16 + 64 deep).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import objectives as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def n_add(V):
+    return V / 256 + 80
+
+
+def randn(shape, dtype, seed, scale=3.0, offset=0.0):
+    g = torch.Generator().manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g) + offset).to(dtype)
+
+
+def np64(t):
+    return t.detach().cpu().double().numpy()
+
+
+def check_scores(got, z, labels, k, temperature=1.0):
+    V = z.shape[-1]
+    z2, y2 = np64(z).reshape(-1, V), None if labels is None else np64(labels).reshape(-1).astype(np.int64)
+    lp, h, ids, top = O.token_logprobs(z2, y2, k, temperature)
+    if labels is not None:
+        d = np64(got.logprobs).reshape(-1)
+        same(d, lp, (n_add(V) + 70 + 4 * np.abs(lp)) * U, "logprobs")
+    if got.entropy is not None:
+        same(np64(got.entropy).reshape(-1), h, np.full(len(h), (n_add(V) + 70) * (1 + np.log2(V + 1)) * U), "entropy")
+    if k:
+        assert np.array_equal(got.top_ids.cpu().numpy().reshape(-1, k), ids)
+        same(np64(got.top_logprobs).reshape(-1, k), top, (n_add(V) + 70 + 4 * np.abs(top)) * U, "top_logprobs")
+
+
+def same(got, want, tol, name):
+    """NaN and infinities where the oracle has them, everything else within tol."""
+    fin = np.isfinite(want)
+    assert np.array_equal(np.isnan(got), np.isnan(want)), name
+    assert np.array_equal(got[~fin & ~np.isnan(want)], want[~fin & ~np.isnan(want)]), name
+    off = np.abs(got[fin] - want[fin]) - tol[fin]
+    assert off.size == 0 or off.max() <= 0, (name, float(off.max()), float(np.abs(got[fin] - want[fin]).max()))
+
+
+def check_grad(got, want, size, dtype, V, extra=1.0):
+    info = torch.finfo(dtype)
+    g = np64(got).reshape(-1, V)
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126       # below it the type has no steps / the kernel flushes
+    tol = (n_add(V) + 82) * U * size * extra + info.eps / 2 * np.abs(want) * (1 + 2 ** -10) + tiny
+    same(g, want, tol, "grad")
+
+
+SHAPES = [(1, 1), (3, 2), (5, 3), (4, 7), (2, 8), (3, 9), (2, 63), (2, 64), (3, 65), (2, 127), (2, 255), (2, 1000), (3, 1025),
+          (2, 4099), (2, 8192), (3, 10000), (2, 16385), (3, 32000), (5, 50021), (2, 65537), (1, 131073), (1, 200019)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows, V", SHAPES)
+def test_scores(rows, V, dtype):
+    from speech_to_text_amd import token_logprobs
+    z = randn((rows, V), TYPES[dtype], 10 * V + rows)
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(V))
+    if rows > 2:
+        y[1] = -100
+    for k in sorted({0, 1, min(V, 5), min(V, 16), min(V, 64)}):
+        got = token_logprobs(z.to(DEV), y.to(DEV), top_k=k, entropy=True)
+        check_scores(got, z, y, k)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows", [1, 2, 7, 64, 255, 300, 1100])
+def test_many_rows(rows, dtype):
+    """From a single decoding step to batches, with padding positions; int32 labels."""
+    from speech_to_text_amd import token_logprobs
+    V = 1009
+    z = randn((rows, V), TYPES[dtype], rows, scale=2.0, offset=30.0)
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(rows), dtype=torch.int32)
+    y[torch.arange(rows) % 5 == 3] = -100
+    got = token_logprobs(z.to(DEV), y.to(DEV), top_k=12, entropy=True, temperature=0.7)
+    check_scores(got, z, y, 12, 0.7)
+
+
+@pytest.mark.parametrize("T", [0.25, 1.0, 2.0, 3.0, 10.0])
+def test_temperature_and_no_labels(T):
+    from speech_to_text_amd import token_logprobs
+    z = randn((3, 5003), torch.bfloat16, 3, scale=4.0, offset=-50.0)
+    got = token_logprobs(z.to(DEV), top_k=9, entropy=True, temperature=T)
+    assert got.logprobs is None
+    check_scores(got, z, None, 9, T)
+    only = token_logprobs(z.to(DEV), entropy=True, temperature=T)
+    assert only.top_ids is None and torch.equal(only.entropy, got.entropy)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_row_strides_and_alignment(dtype):
+    """Slices of positions, batches of a larger vocabulary (rows at every alignment), an expanded batch, more dimensions."""
+    from speech_to_text_amd import token_logprobs
+    t = TYPES[dtype]
+    base = randn((4, 7, 1037), t, 8).to(DEV)
+    y = torch.randint(0, 900, (4, 7), generator=torch.Generator().manual_seed(2)).to(DEV)
+    for z, lab in ((base[:, :-1], y[:, :-1]), (base[:, 1:], y[:, 1:]), (base[..., 3:1003], y), (base[..., 5:6], y * 0),
+                   (base[1:, 2:, 1:1000], y[1:, 2:]), (base[:1].expand(4, 7, 1037), y), (base[:, :1].expand(4, 7, 1037), y),
+                   (base.transpose(0, 1), y.T), (base[0, 0], y[0, 0]), (base.view(2, 2, 7, 1037), y.view(2, 2, 7)),
+                   (base[::2, ::3], y[::2, ::3])):
+        k = min(6, z.shape[-1])
+        got = token_logprobs(z, lab, top_k=k, entropy=True)
+        assert got.logprobs.shape == lab.shape and got.top_ids.shape == lab.shape + (k,)
+        check_scores(got, z.reshape(-1, z.shape[-1]), lab.reshape(-1), k)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [37, 4099, 50021, 131073])
+def test_masked_and_special_rows(V, dtype):
+    """-inf among others, alone, everywhere; the type's lowest value; NaN; +inf; equal values; sorted rows."""
+    from speech_to_text_amd import token_logprobs
+    t = TYPES[dtype]
+    low = torch.finfo(t).min
+    z = randn((16, V), t, V)
+    z[0, ::2] = -np.inf
+    z[1] = -np.inf
+    z[1, V // 3] = 2.0                           # one token left: probability 1, entropy 0
+    z[2] = -np.inf                               # none left
+    z[3] = low                                   # all masked by the lowest value: uniform
+    z[4] = low
+    z[4, V - 1] = 1.0
+    z[5, 7] = np.nan
+    z[6, 5] = np.inf
+    z[7] = 1.5                                   # all equal: the first indices
+    z[8] = torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0).to(t)      # +0 and -0 are equal
+    z[9] = torch.linspace(-8, 8, V).to(t)        # rising: the largest are neighbours
+    z[10] = torch.linspace(8, -8, V).to(t)
+    z[11] = -np.inf
+    z[11, :3] = torch.tensor([0.0, 1.0, 1.0]).to(t)      # fewer finite tokens than alternatives
+    z[12] = np.nan
+    z[13, :] = 0.0
+    z[13, min(V - 1, 20):min(V, 30)] = 4.0       # more equal values than fit between distinct ones
+    z[14] = torch.finfo(t).max
+    z[15] = torch.where(torch.arange(V) % 3 == 0, low, float(z[15, 0])).to(t)
+    y = torch.randint(0, V, (16,), generator=torch.Generator().manual_seed(1))
+    y[0], y[1], y[4], y[5] = 2, V // 3, 0, 7     # a -inf label among them
+    for k in (0, 1, 8, min(V, 64)):
+        check_scores(token_logprobs(z.to(DEV), y.to(DEV), top_k=k, entropy=True), z, y, k)
+
+
+def test_labels_out_of_range_and_custom_ignore():
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    z = randn((5, 300), torch.float32, 4).to(DEV).requires_grad_()
+    y = torch.tensor([300, -1, 7, -100, 2 ** 40]).to(DEV)
+    got = token_logprobs(z, y, entropy=True)
+    assert got.logprobs.isnan().tolist() == [True, True, False, False, True] and not got.entropy.isnan().any()
+    g, = torch.autograd.grad(got.logprobs.sum(), z)
+    assert g.isnan().all(1).tolist() == [True, True, False, False, True] and (g[3] == 0).all()
+    other = token_logprobs(z.detach(), torch.tensor([3, 3, 7, -1, 9]).to(DEV), ignore_index=7)
+    assert other.logprobs.isnan().tolist() == [False, False, False, True, False] and float(other.logprobs[2]) == 0.0
+    ids = torch.tensor([[1, 2], [3, 4], [5, 300], [9, 9], [1, -1]]).to(DEV)
+    y = torch.tensor([300, 5, 7, -100, 2]).to(DEV)
+    loss = distillation_loss(z, y, ids, torch.zeros(5, 2, device=DEV), reduction="none")
+    assert loss.isnan().tolist() == [True, False, True, False, False]
+    g, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    assert g.isnan().all(1).tolist() == [True, False, True, False, False] and not g[[1, 3, 4]].isnan().any()
+
+
+GRAD_SHAPES = [(3, 1), (3, 2), (4, 9), (3, 64), (3, 127), (4, 1000), (3, 4099), (3, 10000), (3, 32000), (4, 50021), (2, 131073)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows, V", GRAD_SHAPES)
+def test_score_gradients(rows, V, dtype):
+    from speech_to_text_amd import token_logprobs
+    t, T, k = TYPES[dtype], 1.3, min(V, 7)
+    z = randn((rows, V), t, V + 1)
+    if V > 8:
+        z[0, 3] = -np.inf
+    g = torch.Generator().manual_seed(V)
+    y = torch.randint(0, V, (rows,), generator=g)
+    y[-1] = -100
+    gl, gh, gt = torch.randn(rows, generator=g), torch.randn(rows, generator=g), torch.randn(rows, k, generator=g)
+    x = z.to(DEV).requires_grad_()
+    out = token_logprobs(x, y.to(DEV), top_k=k, entropy=True, temperature=T)
+    ids = out.top_ids.cpu().numpy()
+    for a, b, c in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+        outs = [o for o, on in zip((out.logprobs, out.entropy, out.top_logprobs), (a, b, c)) if on]
+        ups = [u.to(DEV) for u, on in zip((gl, gh, gt), (a, b, c)) if on]
+        d, = torch.autograd.grad(outs, x, ups, retain_graph=True)
+        assert d.dtype == t and d.shape == x.shape
+        want, size = O.token_logprobs_grad(np64(z), y.numpy(), gl.numpy() if a else None, gh.numpy() if b else None, ids,
+                                           gt.numpy() if c else None, T)
+        # the entropy term p (lp + H) is a difference: its error is that of lp and H, (1 + log2 V) (n_add + 70) u, times p
+        check_grad(d, want, size + (np.abs(gh.numpy())[:, None] * (1 + np.log2(V + 1)) * np.exp(np.nan_to_num(
+            O.log_softmax(np64(z), T), neginf=-1e4)) if b else 0), t, V)
+
+
+def teacher_rows(rows, V, K, seed):
+    """Ids with padding in the middle and the end, a row without any, a row with one id twice, the label among some."""
+    rng = np.random.default_rng(seed)
+    ids = np.stack([rng.permutation(V)[:K] if V >= K else rng.integers(0, V, K) for _ in range(rows)])
+    t = (2 * rng.standard_normal((rows, K))).astype(np.float32)
+    if K > 2:
+        ids[0, 1] = -1
+        ids[-1, K // 2:] = -7
+    if rows > 2:
+        ids[1] = -1
+        ids[2, -1] = ids[2, 0]
+        t[2, 0] = -np.inf if K > 3 else t[2, 0]
+    return torch.from_numpy(ids), torch.from_numpy(t)
+
+
+def check_losses(got, want, z, y, ids, t, tau, alpha):
+    V = z.shape[1]
+    lp1, lpt = O.log_softmax(z), O.log_softmax(z, tau)
+    tol = np.zeros(len(want))
+    for r in range(len(want)):
+        if y[r] < 0 or y[r] >= V or (ids[r] >= V).any():
+            continue
+        q = O.teacher(ids[r], t[r].astype(np.float64), tau)
+        on = q > 0
+        e = np.minimum(n_add(V) + 160 + 4 * (np.abs(lpt[r, ids[r][on]]) + np.abs(np.log(q[on]))), 1e30) * (
+            1 + np.abs(np.log(q[on]) - lpt[r, ids[r][on]])) * q[on]
+        tol[r] = U * (alpha * tau ** 2 * e.sum() + (1 - alpha) * (n_add(V) + 70 + 4 * abs(lp1[r, y[r]])) + 2 * abs(want[r]))
+    same(got, want, tol, "loss")
+    return tol
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows, V, K, tau, alpha", [
+    (3, 1, 1, 1.0, 0.5), (4, 2, 2, 2.0, 0.5), (5, 9, 4, 1.0, 1.0), (4, 64, 64, 2.0, 0.3), (4, 127, 5, 4.0, 0.7), (5, 1000, 16, 2.0, 0.0),
+    (4, 4099, 1, 3.0, 0.5), (4, 10000, 8, 1.0, 0.5), (4, 16385, 20, 1.5, 0.9), (4, 32000, 32, 0.7, 0.5), (5, 50021, 16, 2.0, 0.5),
+    (4, 50021, 64, 4.0, 1.0), (3, 65537, 9, 2.0, 0.8), (3, 131073, 24, 3.0, 0.5), (3, 200019, 64, 2.0, 0.5)])
+def test_distillation(rows, V, K, tau, alpha, dtype):
+    """Loss and gradient, fused ("sum") and per position ("none" with upstream weights), and the loss without a gradient."""
+    from speech_to_text_amd import distillation_loss, distillation_loss_and_grad
+    t = TYPES[dtype]
+    z = randn((rows, V), t, 7 * V + K)
+    g = torch.Generator().manual_seed(K)
+    y = torch.randint(0, V, (rows,), generator=g)
+    ids, teacher = teacher_rows(rows, V, K, V + K)
+    y[0] = max(0, int(ids[0, 0]))
+    if rows > 3:
+        y[3] = -100
+    want, grad, size = O.distillation(np64(z), y.numpy(), ids.numpy(), teacher.numpy(), tau, alpha)
+    x = z.to(DEV).requires_grad_()
+    args = (y.to(DEV), ids.to(DEV), teacher.to(DEV))
+    kw = dict(temperature=tau, alpha=alpha)
+    each = distillation_loss(x, *args, reduction="none", **kw)
+    tol = check_losses(np64(each), want, np64(z), y.numpy(), ids.numpy(), teacher.numpy(), tau, alpha)
+    with torch.no_grad():
+        assert torch.equal(distillation_loss(x, *args, reduction="none", **kw), each)
+    w = torch.randn(rows, generator=g)
+    d, = torch.autograd.grad(each, x, w.to(DEV))
+    check_grad(d, grad * w.numpy()[:, None], size * np.abs(w.numpy())[:, None], t, V)
+    n = int((y != -100).sum())
+    for red, f in (("sum", 1.0), ("mean", 1.0 / n)):
+        total = distillation_loss(x, *args, reduction=red, **kw)
+        d, = torch.autograd.grad(total, x)
+        total = total.detach()
+        assert abs(float(total) - want.sum() * f) <= (tol.sum() + 4 * U * np.abs(want).sum()) * f
+        check_grad(d, grad * f, size * f, t, V)
+        loss2, d2 = distillation_loss_and_grad(x, *args, reduction=red, **kw)
+        assert abs(float(loss2) - float(total)) <= 2 * (tol.sum() + 4 * U * np.abs(want).sum()) * f
+        check_grad(d2, grad * f, size * f, t, V)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_distillation_specials(dtype):
+    """Student logits of -inf (at a teacher's id: loss +inf), rows of the lowest value, of only -inf, NaN, +inf."""
+    from speech_to_text_amd import distillation_loss
+    t = TYPES[dtype]
+    V, K = 4099, 3
+    z = randn((8, V), t, 5)
+    ids = torch.tensor([[1, 2, 3]] * 8)
+    z[0, 2] = -np.inf                             # a kept entry the student rules out
+    z[1, 100:] = -np.inf
+    z[2] = torch.finfo(t).min
+    z[3] = -np.inf
+    z[4, 9] = np.nan
+    z[5, 9] = np.inf
+    teacher = torch.tensor([[0.0, -1.0, -2.0]] * 8)
+    teacher[6] = -np.inf                          # entries without weight: no teacher term
+    ids[7] = -1
+    y = torch.tensor([1, 5, 7, 1, 2, 2, 3, 4])
+    want, grad, size = O.distillation(np64(z), y.numpy(), ids.numpy(), teacher.numpy(), 2.0, 0.5)
+    assert np.isposinf(want[0]) and np.isfinite(want[[1, 2, 6, 7]]).all() and np.isnan(want[[3, 4, 5]]).all()
+    x = z.to(DEV).requires_grad_()
+    each = distillation_loss(x, y.to(DEV), ids.to(DEV), teacher.to(DEV), temperature=2.0, reduction="none")
+    check_losses(np64(each), want, np.nan_to_num(np64(z), nan=0, neginf=-1e4), y.numpy(), ids.numpy(), teacher.numpy(), 2.0, 0.5)
+    d, = torch.autograd.grad(each, x, torch.ones(8, device=DEV))
+    check_grad(d, grad, size, t, V)
+    d, = torch.autograd.grad(distillation_loss(x, y.to(DEV), ids.to(DEV), teacher.to(DEV), temperature=2.0, reduction="sum"), x)
+    check_grad(d, grad, size, t, V)
+
+
+def test_strided_student_and_types_of_the_teacher():
+    from speech_to_text_amd import distillation_loss
+    base = randn((3, 6, 2049), torch.bfloat16, 6).to(DEV)
+    x = base[:, :-1, 1:].detach().requires_grad_()
+    y = torch.randint(0, 2048, (3, 5), generator=torch.Generator().manual_seed(3))
+    y[0, 3:] = -100
+    ids, t = teacher_rows(15, 2048, 6, 1)
+    t = t.to(torch.bfloat16)
+    want, grad, size = O.distillation(np64(x).reshape(15, -1), y.numpy().reshape(-1), ids.numpy(), t.float().numpy(), 2.0, 0.4)
+    loss = distillation_loss(x, y.int().to(DEV), ids.int().view(3, 5, 6).to(DEV), t.view(3, 5, 6).to(DEV), temperature=2.0, alpha=0.4)
+    d, = torch.autograd.grad(loss, x)
+    assert d.shape == x.shape and d.is_contiguous()
+    check_grad(d, grad / 13, size / 13, torch.bfloat16, 2048)
+    # one student row for every position: autograd sums the positions' gradients
+    row = base[0, 0, 1:].detach().float().requires_grad_()
+    loss = distillation_loss(row.expand(3, 5, 2048), y.to(DEV), ids.view(3, 5, 6).to(DEV), t.float().view(3, 5, 6).to(DEV), reduction="sum")
+    d, = torch.autograd.grad(loss, row)
+    _, grad, size = O.distillation(np.broadcast_to(np64(row), (15, 2048)), y.numpy().reshape(-1), ids.numpy(), t.float().numpy())
+    check_grad(d, grad.sum(0, keepdims=True), size.sum(0, keepdims=True), torch.float32, 2048)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_backward_twice_and_upstream_factors(dtype):
+    """A graph that is kept gives the same gradient again, whatever the first upstream gradient was; the loss stays usable."""
+    from speech_to_text_amd import distillation_loss
+    z = randn((6, 3001), TYPES[dtype], 9)
+    y = torch.randint(0, 3001, (6,), generator=torch.Generator().manual_seed(9))
+    ids, t = teacher_rows(6, 3001, 5, 2)
+    want, grad, size = O.distillation(np64(z), y.numpy(), ids.numpy(), t.numpy())
+    x = z.to(DEV).requires_grad_()
+    loss = distillation_loss(x, y.to(DEV), ids.to(DEV), t.to(DEV), weight=0.25)
+    first, = torch.autograd.grad(loss, x, torch.tensor(3.0, device=DEV), retain_graph=True)
+    kept = first.clone()
+    second, = torch.autograd.grad(loss, x, torch.tensor(-1.0, device=DEV), retain_graph=True)
+    loss.mul_(2.0)                                 # the caller's tensor, not the graph's
+    f = 0.25 / 6
+    assert torch.equal(first, kept)
+    # an upstream factor rounds the made gradient a second time (bf16 / fp32): one more half step
+    tol_twice = 2.0 if dtype != "fp16" else 1.0
+    for d, g in ((first, 3.0), (second, -1.0)):
+        info = torch.finfo(TYPES[dtype])
+        w = grad * f * g
+        tol = (n_add(3001) + 82) * U * size * f * abs(g) + tol_twice * info.eps / 2 * np.abs(w) * (1 + 2 ** -6) + 2 ** -24
+        same(np64(d), w, tol, "grad")
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(torch.autograd.grad(distillation_loss(x, y.to(DEV), ids.to(DEV), t.to(DEV)), x, create_graph=True)[0].sum(), x)
+
+
+def test_no_rows_that_count():
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    x = randn((4, 99), torch.float32, 1).to(DEV).requires_grad_()
+    y = torch.full((4,), -100, device=DEV)
+    ids, t = torch.full((4, 3), -1, device=DEV), torch.zeros(4, 3, device=DEV)
+    loss = distillation_loss(x, y, ids, t)
+    d, = torch.autograd.grad(loss, x)
+    assert float(loss) == 0.0 and (d == 0).all()
+    e = x[:0]
+    loss = distillation_loss(e, y[:0], ids[:0], t[:0])
+    d, = torch.autograd.grad(loss, x)
+    assert float(loss) == 0.0 and (d == 0).all()
+    assert distillation_loss(e.detach(), y[:0], ids[:0], t[:0], reduction="none").shape == (0,)
+    s = token_logprobs(e.detach(), y[:0], top_k=2, entropy=True)
+    assert s.logprobs.shape == (0,) and s.top_ids.shape == (0, 2)
+    s = token_logprobs(x.detach(), y, top_k=2, entropy=True)
+    assert (s.logprobs == 0).all() and (s.entropy == 0).all() and (s.top_ids == -1).all() and (s.top_logprobs == -np.inf).all()
+
+
+def test_gradients_against_differences():
+    """Central differences of the kernels' own losses along random directions: with h = 2^-5 and third derivatives along a unit
+    direction below 1, |difference - slope| <= h^2 / 6 + (error of a loss, n_add + 250 u times its size) / h."""
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    rows, V, h = 4, 37, 2.0 ** -5
+    z = randn((rows, V), torch.float32, 11, scale=1.0)
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(8)).to(DEV)
+    ids, t = (a.to(DEV) for a in teacher_rows(rows, V, 4, 3))
+
+    def score(x):
+        s = token_logprobs(x, y, top_k=3, entropy=True, temperature=1.5)
+        return (s.logprobs + 0.5 * s.entropy + 0.1 * s.top_logprobs.sum(-1)).sum()
+
+    def distil(x):
+        return distillation_loss(x, y, ids, t, temperature=1.5, alpha=0.6, reduction="sum")
+
+    for f in (score, distil):
+        x = z.to(DEV).requires_grad_()
+        slope, = torch.autograd.grad(f(x), x)
+        for seed in range(4):
+            v = randn((rows, V), torch.float32, 100 + seed)
+            v = (v / v.norm()).to(DEV)
+            with torch.no_grad():
+                up, down = f(x + h * v), f(x - h * v)
+            diff = (float(up) - float(down)) / (2 * h)
+            assert abs(diff - float((slope * v).sum())) <= h * h / 6 + 350 * U * max(abs(float(up)), 10.0) / h
+
+
+def test_far_rows():
+    """Rows behind 2^31 elements and 2^32 bytes."""
+    from speech_to_text_amd import distillation_loss_and_grad, token_logprobs
+    B, P, V = 35, 2000, 32003                      # 2.24e9 elements, 4.48e9 bytes
+    z = torch.zeros((B, P, V), dtype=torch.bfloat16, device=DEV)
+    z[-1, -3:] = randn((3, V), torch.bfloat16, 1).to(DEV)
+    y = torch.full((B, P), -100, device=DEV)
+    y[-1, -3:] = torch.tensor([5, 31000, 32002], device=DEV)
+    y[0, 0] = 1
+    ids = torch.full((B, P, 4), -1, device=DEV)
+    ids[-1, -3:] = torch.tensor([5, 9, 32002, 20000], device=DEV)
+    t = torch.zeros((B, P, 4), device=DEV)
+    s = token_logprobs(z, y, top_k=4, entropy=True)
+    check_scores(type(s)(*(a[-1, -3:] for a in s)), z[-1, -3:], y[-1, -3:], 4)
+    check_scores(type(s)(*(a[0, :2] for a in s)), z[0, :2], y[0, :2], 4)
+    _, g = distillation_loss_and_grad(z, y, ids, t, temperature=2.0, reduction="sum")
+    _, grad, size = O.distillation(np64(z[-1, -3:]), y[-1, -3:].cpu().numpy(), ids[-1, -3:].cpu().numpy(), t[-1, -3:].cpu().numpy(), 2.0)
+    check_grad(g[-1, -3:], grad, size, torch.bfloat16, V)
+    assert (g[-1, :-3] == 0).all() and (g[1:3] == 0).all()
+
+
+def test_results_repeat_and_neighbours_stay():
+    """Twice the same bits, with and without the other outputs asked for; a view's surroundings are not written."""
+    from speech_to_text_amd import _lib, distillation_loss_and_grad, token_logprobs
+    z = randn((300, 5003), torch.bfloat16, 2).to(DEV)
+    y = torch.randint(0, 5003, (300,), generator=torch.Generator().manual_seed(4)).to(DEV)
+    a, b = token_logprobs(z, y, top_k=20, entropy=True), token_logprobs(z, y, top_k=20, entropy=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    c = token_logprobs(z, y)
+    assert torch.equal(c.logprobs, a.logprobs)
+    ids, t = (v.to(DEV) for v in teacher_rows(300, 5003, 8, 5))
+    p, q = distillation_loss_and_grad(z, y, ids, t), distillation_loss_and_grad(z, y, ids, t)
+    assert torch.equal(p[0], q[0]) and torch.equal(p[1], q[1])
+    # through the C ABI: a gradient that starts and ends inside a larger buffer, at an odd element
+    for dtype, code in ((torch.bfloat16, 2), (torch.float16, 1), (torch.float32, 0)):
+        zz = z.to(dtype)
+        buf = torch.full((300 * 5003 + 34,), 7.0, dtype=dtype, device=DEV)
+        out = buf[17:-17]
+        losses, stats = torch.empty(300, device=DEV), torch.empty(300, 4, device=DEV)
+        st = torch.cuda.current_stream().cuda_stream
+        n = __import__("ctypes").c_size_t()
+        _lib.check(_lib.lib().sttfe_distill_workspace_bytes(300, 5003, code, __import__("ctypes").byref(n)))
+        ws = torch.empty(max(n.value, 1), dtype=torch.uint8, device=DEV)
+        P = _lib.ptr
+        _lib.check(_lib.lib().sttfe_distill_loss(P(zz), code, 1, 300, 0, 5003, 5003, P(y), -100, P(ids), P(t), 8, 1.0, 0.5, 1.0, 0,
+                                                 P(losses), None, None, P(stats), P(out), P(ws), n.value, st))
+        _, want = distillation_loss_and_grad(zz, y, ids, t, reduction="sum")
+        assert torch.equal(out.view(300, 5003), want) and (buf[:17] == 7).all() and (buf[-17:] == 7).all()
+
+
+def test_another_stream():
+    from speech_to_text_amd import distillation_loss_and_grad, token_logprobs
+    z = randn((64, 50021), torch.bfloat16, 3).to(DEV)
+    y = torch.randint(0, 50021, (64,), generator=torch.Generator().manual_seed(4)).to(DEV)
+    ids, t = (v.to(DEV) for v in teacher_rows(64, 50021, 8, 5))
+    want, grad = token_logprobs(z, y, top_k=5, entropy=True), distillation_loss_and_grad(z, y, ids, t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got, g2 = token_logprobs(z, y, top_k=5, entropy=True), distillation_loss_and_grad(z, y, ids, t)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(want, got)) and torch.equal(grad[1], g2[1])
+
+
+@pytest.mark.parametrize("rows, V", [(1, 50021), (40, 10000), (300, 5003), (3, 200019)])
+def test_captured_graphs(rows, V):
+    """Two captured graphs (a decoding step's scores, a training step's loss and gradient) replayed in turn on new inputs."""
+    from speech_to_text_amd import distillation_loss_and_grad, token_logprobs
+    z = randn((rows, V), torch.bfloat16, 0).to(DEV)
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(4)).to(DEV)
+    ids, t = (v.to(DEV) for v in teacher_rows(rows, V, 8, 5))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        token_logprobs(z, y, top_k=5, entropy=True), distillation_loss_and_grad(z, y, ids, t)
+    torch.cuda.current_stream().wait_stream(side)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        a = token_logprobs(z, y, top_k=5, entropy=True)
+    with torch.cuda.graph(g2):
+        b = distillation_loss_and_grad(z, y, ids, t)
+    for k in range(4):
+        z.copy_(randn((rows, V), torch.bfloat16, 20 + k).to(DEV))
+        y.copy_(torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(50 + k)).to(DEV))
+        g1.replay()
+        g2.replay()
+        torch.cuda.synchronize()
+        want, (loss, grad) = token_logprobs(z, y, top_k=5, entropy=True), distillation_loss_and_grad(z, y, ids, t)
+        assert all(torch.equal(p, q) for p, q in zip(a, want))
+        assert torch.equal(b[0], loss) and torch.equal(b[1], grad)
+
+
+def test_teacher_to_student(tmp_path):
+    """The run as it is used: a teacher's logits over a batch go to the cache (token_logprobs on the GPU), come back through
+    dataset and collator, and the student's gradient is the oracle's for those alternatives; the alternatives are a softmax's."""
+    from speech_to_text_amd import AudioCollator, DataConfig, FeatureCacheDataset, FeatureCacheWriter, distillation_loss, token_logprobs
+    B, V, K = 5, 10007, 12
+    rng = np.random.default_rng(0)
+    labels = [rng.integers(0, V, n).tolist() for n in (7, 1, 12, 0, 5)]
+    teacher = randn((B, 14, V), torch.bfloat16, 1).to(DEV)
+    w = FeatureCacheWriter(str(tmp_path), "speech2text", 80, shard_clips=2, teacher_top=K)
+    w.add_batch(list(range(B)), torch.zeros(B, 80, 30), [0] * B, labels=labels, teacher_logits=teacher)
+    w.close()
+    ds = FeatureCacheDataset(str(tmp_path))
+    batch = AudioCollator(DataConfig(), "speech2text", True)([ds[i] for i in range(B)])
+    y, ids, t = batch["labels"], batch["teacher_ids"], batch["teacher_logits"]
+    assert y.shape == (B, 12) and ids.shape == (B, 12, K)
+    for b in range(B):
+        n = len(labels[b])
+        _, _, want, top = O.token_logprobs(np64(teacher[b, :n]), None, K)
+        assert np.array_equal(ids[b, :n].numpy(), want)
+        same(np64(t[b, :n]), top, (n_add(V) + 70 + 4 * np.abs(top)) * U, "kept")
+    z = randn((B, 12, V), torch.bfloat16, 2)
+    x = z.to(DEV).requires_grad_()
+    loss = distillation_loss(x, y.to(DEV), ids.to(DEV), t.to(DEV), temperature=2.0, alpha=0.8)
+    loss.backward()
+    want, grad, size = O.distillation(np64(z).reshape(-1, V), y.numpy().reshape(-1), ids.numpy().reshape(-1, K),
+                                      t.numpy().reshape(-1, K), 2.0, 0.8)
+    n = sum(map(len, labels))
+    tol = check_losses(want, want, np64(z).reshape(-1, V), y.numpy().reshape(-1), ids.numpy().reshape(-1, K), t.numpy().reshape(-1, K), 2.0, 0.8)
+    assert abs(float(loss.detach()) - want.sum() / n) <= (tol.sum() + 4 * U * np.abs(want).sum()) / n
+    check_grad(x.grad, grad / n, size / n, torch.bfloat16, V)
+    # the same labels scored by the student: the loss without a teacher is the mean of the label's -logprob
+    s = token_logprobs(x.detach(), y.to(DEV))
+    ce = distillation_loss(x.detach(), y.to(DEV), ids.to(DEV), t.to(DEV), alpha=0.0)
+    assert abs(float(ce) + float(s.logprobs.double().sum()) / n) <= 4 * U * abs(float(ce)) + 2 * (n_add(V) + 70) * U
