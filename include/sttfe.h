@@ -317,7 +317,7 @@ int sttfe_pitch_shift(float* pcm, const int64_t* offsets, const int32_t* lengths
 #define STTFE_DTYPE_BF16 2
 #define STTFE_MAX_TOP 64                 /* alternatives per row */
 #define STTFE_MAX_ROWS 16777216
-#define STTFE_MAX_VOCAB 4194304
+#define STTFE_MAX_VOCAB 2097152
 #define STTFE_REDUCE_NONE 0
 #define STTFE_REDUCE_SUM 1
 #define STTFE_REDUCE_MEAN 2
