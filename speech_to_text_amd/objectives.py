@@ -97,32 +97,44 @@ def _temperature(temperature: float, what: str) -> float:
     return temperature
 
 
-def _stream(device: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _call(name: str, device: torch.device, *args):
+    """One entry point of the library on the device's current stream.
+
+    The host side of a small training step costs more than its kernels: the stream comes as a number (building a Stream object
+    takes 4 us, and 15 when the autograd thread builds them too), the device is only changed if it is another."""
+    fn = getattr(_lib.lib(), name)
+    if torch._C._cuda_getDevice() == device.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != 0:
+        _lib.check(rc, name)
 
 
 def _workspace(name: str, device: torch.device, *args) -> Tuple[Optional[torch.Tensor], int]:
     n = ctypes.c_size_t()
-    _lib.check(getattr(_lib.lib(), name)(*args, ctypes.byref(n)), name)
-    if n.value == 0:
-        return None, 0
-    return torch.empty(n.value, dtype=torch.uint8, device=device), n.value
+    rc = getattr(_lib.lib(), name)(*args, ctypes.byref(n))
+    if rc != 0:
+        _lib.check(rc, name)
+    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
 
 
 # ------------------------------------------------------------------------------------------------- token_logprobs
 def _logprobs_forward(logits, rows, labels, top_k, want_entropy, temperature, ignore_index, want_stats):
     device, lead = logits.device, logits.shape[:-1]
-    f32 = dict(dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        logprobs = torch.empty(lead, **f32) if labels is not None else None
-        entropy = torch.empty(lead, **f32) if want_entropy else None
-        stats = torch.empty(lead + (4,), **f32) if want_stats else None
-        ids = torch.empty(lead + (top_k,), dtype=torch.int64, device=device) if top_k else None
-        top = torch.empty(lead + (top_k,), **f32) if top_k else None
-        ws, n = _workspace("sttfe_token_logprobs_workspace_bytes", device, rows[2] * rows[3], rows[6], rows[1], top_k)
-        p = _lib.ptr
-        _lib.check(_lib.lib().sttfe_token_logprobs(*rows, p(labels), ignore_index, temperature, top_k, p(logprobs), p(entropy),
-                                                   p(stats), p(ids), p(top), p(ws), n, _stream(device)), "sttfe_token_logprobs")
+    logprobs = torch.empty(lead, dtype=torch.float32, device=device) if labels is not None else None
+    entropy = torch.empty(lead, dtype=torch.float32, device=device) if want_entropy else None
+    stats = torch.empty(lead + (4,), dtype=torch.float32, device=device) if want_stats else None
+    ids = torch.empty(lead + (top_k,), dtype=torch.int64, device=device) if top_k else None
+    top = torch.empty(lead + (top_k,), dtype=torch.float32, device=device) if top_k else None
+    ws, n = _workspace("sttfe_token_logprobs_workspace_bytes", device, rows[2] * rows[3], rows[6], rows[1], top_k)
+    _call("sttfe_token_logprobs", device, *rows, _ptr(labels), ignore_index, temperature, top_k, _ptr(logprobs), _ptr(entropy),
+          _ptr(stats), _ptr(ids), _ptr(top), _ptr(ws), n)
     return logprobs, entropy, ids, top, stats
 
 
@@ -145,15 +157,11 @@ class _TokenLogprobs(torch.autograd.Function):
         if g_logprobs is None and g_entropy is None and g_top is None:
             return (None,) * 7
         top_k, temperature, ignore_index = ctx.args
-        device = logits.device
         rows = _rows(logits, "token_logprobs")
-        with torch.cuda.device(device):
-            g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_logprobs, g_entropy, g_top)]
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-            p = _lib.ptr
-            _lib.check(_lib.lib().sttfe_token_logprobs_grad(*rows, p(labels), ignore_index, temperature, p(stats), p(g[0]), p(g[1]),
-                                                            top_k, p(ids), p(g[2]), p(grad), _stream(device)),
-                       "sttfe_token_logprobs_grad")
+        g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_logprobs, g_entropy, g_top)]
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _call("sttfe_token_logprobs_grad", logits.device, *rows, _ptr(labels), ignore_index, temperature, _ptr(stats), _ptr(g[0]),
+              _ptr(g[1]), top_k, _ptr(ids), _ptr(g[2]), _ptr(grad))
         return grad, None, None, None, None, None, None
 
 
@@ -212,30 +220,27 @@ def _distill_args(what, logits, labels, teacher_ids, teacher_logits, temperature
 
 
 def _distill_forward(logits, args, want_stats, want_grad):
+    """-> loss, factor, stats, gradient (each None if not wanted; the factor with the stats only)."""
     rows, labels, ids, teacher, K, temperature, alpha, ignore_index, weight, reduction = args
     device, lead = logits.device, logits.shape[:-1]
-    f32 = dict(dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        losses = torch.empty(lead, **f32)
-        total, factor = (torch.empty((), **f32), torch.empty((), **f32)) if reduction != "none" else (None, None)
-        stats = torch.empty(lead + (4,), **f32) if want_stats else None
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
-        ws, n = _workspace("sttfe_distill_workspace_bytes", device, rows[2] * rows[3], rows[6], rows[1])
-        p = _lib.ptr
-        _lib.check(_lib.lib().sttfe_distill_loss(*rows, p(labels), ignore_index, p(ids), p(teacher), K, temperature, alpha, weight,
-                                                 _REDUCE[reduction], p(losses), p(total), p(factor), p(stats), p(grad), p(ws), n,
-                                                 _stream(device)), "sttfe_distill_loss")
+    f32 = torch.float32
+    losses = torch.empty(lead, dtype=f32, device=device)
+    total = factor = None
+    if reduction != "none":
+        total, factor = torch.empty((), dtype=f32, device=device), torch.empty((), dtype=f32, device=device)
+    stats = torch.empty(lead + (4,), dtype=f32, device=device) if want_stats else None
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device) if want_grad else None
+    ws, n = _workspace("sttfe_distill_workspace_bytes", device, rows[2] * rows[3], rows[6], rows[1])
+    _call("sttfe_distill_loss", device, *rows, _ptr(labels), ignore_index, _ptr(ids), _ptr(teacher), K, temperature, alpha, weight,
+          _REDUCE[reduction], _ptr(losses), _ptr(total), _ptr(factor), _ptr(stats), _ptr(grad), _ptr(ws), n)
     return losses if total is None else total, factor, stats, grad
 
 
 def _distill_backward(logits, args, stats, factor, g, g_rows):
     rows, labels, ids, teacher, K, temperature, alpha, ignore_index, weight, reduction = args
-    device = logits.device
-    with torch.cuda.device(device):
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-        p = _lib.ptr
-        _lib.check(_lib.lib().sttfe_distill_grad(*rows, p(labels), ignore_index, p(ids), p(teacher), K, temperature, alpha, p(stats),
-                                                 p(factor), p(g), p(g_rows), p(grad), _stream(device)), "sttfe_distill_grad")
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    _call("sttfe_distill_grad", logits.device, *rows, _ptr(labels), ignore_index, _ptr(ids), _ptr(teacher), K, temperature, alpha,
+          _ptr(stats), _ptr(factor), _ptr(g), _ptr(g_rows), _ptr(grad))
     return grad
 
 
@@ -247,27 +252,24 @@ class _Distillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, args):
-        reduction = args[-1]
-        fused = reduction != "none" and logits.dtype != torch.float16
-        loss, factor, stats, grad = _distill_forward(logits, args, True, fused)
+        fused = args[-1] != "none" and logits.dtype != torch.float16
+        loss, factor, stats, ctx.grad = _distill_forward(logits, args, not fused, fused)
         ctx.scalars = args[4:]
-        ctx.grad = grad
-        ctx.save_for_backward(logits, *args[1:4], stats, factor)
+        ctx.save_for_backward(logits, *args[1:4], stats, None if fused else factor)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, labels, ids, teacher, stats, factor = ctx.saved_tensors
-        device = logits.device
         g = g.to(torch.float32).contiguous()
         grad, ctx.grad = ctx.grad, None                 # handed out once: a second pass over a kept graph computes its own
         if grad is not None:
-            with torch.cuda.device(device):
-                _lib.check(_lib.lib().sttfe_distill_rescale(_lib.ptr(grad), _DTYPES[grad.dtype], grad.numel(), _lib.ptr(g),
-                                                            _stream(device)), "sttfe_distill_rescale")
+            _call("sttfe_distill_rescale", grad.device, _ptr(grad), _DTYPES[grad.dtype], grad.numel(), _ptr(g))
             return grad, None
         args = (_rows(logits, "distillation_loss"), labels, ids, teacher) + ctx.scalars
+        if stats is None:
+            _, factor, stats, _ = _distill_forward(logits, args, True, False)
         if args[-1] == "none":
             return _distill_backward(logits, args, stats, None, None, g), None
         return _distill_backward(logits, args, stats, factor, g, None), None
