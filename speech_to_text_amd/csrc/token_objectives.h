@@ -68,8 +68,12 @@ struct Distill {
     bool teacher, label;                         // which terms there are
 };
 
+__host__ __device__ inline float mean_factor(float weight, int rows) { return (float)((double)weight / (double)(rows ? rows : 1)); }
+constexpr int kCountHere = 1024;   // up to this many rows a mean's teams count the rows themselves: a launch less
 struct Out {
-    const float* factor;
+    const float* factor;           // what the gradient is multiplied by; NULL: by weight, or (mean) weight / rows that count
+    float weight;
+    bool mean;
     float *losses, *stats;
     float4* parts;
     uint32_t rows;

@@ -11,13 +11,11 @@ namespace sttfe {
 namespace {
 
 
-// factor = weight (sum) or weight / number of rows that count (mean)
+// Rows that count, by one team.
 constexpr int kRowsThreads = 1024;
-__global__ __launch_bounds__(kRowsThreads) void distill_factor_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t rows,
-                                                                      float weight, int mean, float* __restrict__ factor) {
-    __shared__ int part[kRowsThreads / 64];
+__device__ int count_rows(const int64_t* __restrict__ labels, int64_t ignore, int64_t rows, int* part) {
     int n = 0;                                   // at most 2^24 rows
-    for (int64_t r0 = 0; mean && r0 < rows; r0 += 8 * kRowsThreads)
+    for (int64_t r0 = 0; r0 < rows; r0 += 8 * kRowsThreads)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int64_t r = r0 + i * kRowsThreads + threadIdx.x;
@@ -26,17 +24,29 @@ __global__ __launch_bounds__(kRowsThreads) void distill_factor_kernel(const int6
         }
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int all = 0;
-        for (int i = 0; i < kRowsThreads / 64; ++i) all += part[i];
-        factor[0] = mean ? (float)((double)weight / (double)(all ? all : 1)) : weight;
-    }
+    n = 0;
+    for (int i = 0; i < kRowsThreads / 64; ++i) n += part[i];
+    return n;
+}
+
+// factor = weight (sum) or weight / number of rows that count (mean)
+__global__ __launch_bounds__(kRowsThreads) void distill_factor_kernel(const int64_t* __restrict__ labels, int64_t ignore, int64_t rows,
+                                                                      float weight, bool mean, float* __restrict__ factor) {
+    __shared__ int part[kRowsThreads / 64];
+    const int n = mean ? count_rows(labels, ignore, rows, part) : 1;
+    if (threadIdx.x == 0) factor[0] = mean_factor(weight, n);
 }
 
 // total = factor * sum of the rows' losses, in 64 bits and in a fixed order
+enum Factor { kFactorMade = 0, kFactorWeight = 1, kFactorCount = 2 };      // where the factor comes from
 __global__ __launch_bounds__(kRowsThreads) void distill_total_kernel(const float* __restrict__ losses, int64_t rows,
-                                                                     const float* __restrict__ factor, float* __restrict__ total) {
+                                                                     const int64_t* __restrict__ labels, int64_t ignore, float weight,
+                                                                     int from, float* __restrict__ factor, float* __restrict__ total) {
+    __shared__ int part_n[kRowsThreads / 64];
     __shared__ double part[kRowsThreads / 64];
+    float f = weight;
+    if (from == kFactorCount) f = mean_factor(weight, count_rows(labels, ignore, rows, part_n));
+    if (from == kFactorMade) f = factor[0];
     double s = 0.0;
     for (int64_t r0 = 0; r0 < rows; r0 += 8 * kRowsThreads)
 #pragma unroll
@@ -51,7 +61,8 @@ __global__ __launch_bounds__(kRowsThreads) void distill_total_kernel(const float
     if (threadIdx.x == 0) {
         double all = 0.0;
         for (int i = 0; i < kRowsThreads / 64; ++i) all += part[i];
-        total[0] = (float)(all * (double)factor[0]);
+        total[0] = (float)(all * (double)f);
+        factor[0] = f;
     }
 }
 
@@ -69,9 +80,9 @@ int compute_units() {
 // Teams of a launch over n rows: 0 = one for every segment, else that many which deal the rows among themselves: as many as the
 // registers of two rows a thread leave room for.
 int dealt_teams(const Plan& plan, int64_t n, bool ahead) {
-    if (plan.segs > 1 || kTeamWaves[plan.team] < 4) return 0;
+    if (kTeamWaves[plan.team] < 4) return 0;
     const int teams = compute_units() * (4 * kWavesPerSimd(kTeamVpt[plan.team], ahead) / kTeamWaves[plan.team]);
-    return n > teams ? teams : 0;
+    return n * plan.segs > teams ? teams : 0;
 }
 
 Distill distill_args(const int64_t* labels, int64_t ignore, const int64_t* ids, const float* teacher, int K, float tau, float alpha) {
@@ -212,22 +223,26 @@ extern "C" int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, 
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     const Distill a = distill_args(labels, ignore_index, teacher_ids, teacher_logits, teacher_k, temperature, alpha);
     const Mode mode = distill_mode(a);
-    const float* made = reduction != STTFE_REDUCE_NONE ? factor : nullptr;
-    if (reduction != STTFE_REDUCE_NONE)
-        hipLaunchKernelGGL(distill_factor_kernel, dim3(1), dim3(kRowsThreads), 0, stream, labels, ignore_index, n, weight,
-                           reduction == STTFE_REDUCE_MEAN ? 1 : 0, factor);
+    // The factor of the gradient: from a kernel of its own where there are many rows to count, or a gradient kernel to read it.
+    const bool mean = reduction == STTFE_REDUCE_MEAN, apart = grad && plan.segs > 1;
+    const Factor from = reduction == STTFE_REDUCE_NONE ? kFactorWeight
+                        : apart || (mean && n > kCountHere) ? kFactorMade : mean ? kFactorCount : kFactorWeight;
+    if (from == kFactorMade)
+        hipLaunchKernelGGL(distill_factor_kernel, dim3(1), dim3(kRowsThreads), 0, stream, labels, ignore_index, n, weight, mean, factor);
+    const float* made = from == kFactorMade ? factor : nullptr;
+    const float sum_weight = reduction == STTFE_REDUCE_NONE ? 1.f : weight;
     if (n > 0) {
         ScopedTiming t(kTimeDistill, stream);
         float4* parts = static_cast<float4*>(workspace);
         const int teams = dealt_teams(plan, n, kDistillAhead);
-        const Out o{made, losses, stats, parts, (uint32_t)n, teams > 0};
+        const Out o{made, sum_weight, mean, losses, stats, parts, (uint32_t)n, teams > 0};
         if (plan.segs == 1) {
             STTFE_BY_DTYPE(dtype, Launch<T>::distill(plan, rows, a, mode, (unsigned)(teams ? teams : n), o, static_cast<T*>(grad), stream));
         } else {
             // a row over several teams: their sums, the loss from the joined sums, then the gradient in a pass of its own
             float* st = stats ? stats : reinterpret_cast<float*>(parts + n * plan.segs);
             STTFE_BY_DTYPE(dtype, {
-                Launch<T>::distill(plan, rows, a, mode, (unsigned)(n * plan.segs), o, static_cast<T*>(nullptr), stream);
+                Launch<T>::distill(plan, rows, a, mode, (unsigned)(teams ? teams : n * plan.segs), o, static_cast<T*>(nullptr), stream);
                 Launch<T>::distill_join(rows, a, mode, parts, losses, st, (unsigned)n, stream);
             });
             if (grad) {
@@ -239,7 +254,8 @@ extern "C" int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, 
         }
     }
     if (reduction != STTFE_REDUCE_NONE)
-        hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(kRowsThreads), 0, stream, losses, n, factor, total);
+        hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(kRowsThreads), 0, stream, losses, n, labels, ignore_index, weight,
+                           (int)from, factor, total);
     if (hip_failed(hipGetLastError(), "distillation kernel launch")) return STTFE_E_LAUNCH;
     return STTFE_OK;
 }

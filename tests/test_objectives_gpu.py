@@ -362,11 +362,11 @@ def test_no_rows_that_count():
     ids, t = torch.full((4, 3), -1, device=DEV), torch.zeros(4, 3, device=DEV)
     loss = distillation_loss(x, y, ids, t)
     d, = torch.autograd.grad(loss, x)
-    assert float(loss) == 0.0 and (d == 0).all()
+    assert float(loss.detach()) == 0.0 and (d == 0).all()
     e = x[:0]
     loss = distillation_loss(e, y[:0], ids[:0], t[:0])
     d, = torch.autograd.grad(loss, x)
-    assert float(loss) == 0.0 and (d == 0).all()
+    assert float(loss.detach()) == 0.0 and (d == 0).all()
     assert distillation_loss(e.detach(), y[:0], ids[:0], t[:0], reduction="none").shape == (0,)
     s = token_logprobs(e.detach(), y[:0], top_k=2, entropy=True)
     assert s.logprobs.shape == (0,) and s.top_ids.shape == (0, 2)
@@ -528,3 +528,76 @@ def test_teacher_to_student(tmp_path):
     s = token_logprobs(x.detach(), y.to(DEV))
     ce = distillation_loss(x.detach(), y.to(DEV), ids.to(DEV), t.to(DEV), alpha=0.0)
     assert abs(float(ce) + float(s.logprobs.double().sum()) / n) <= 4 * U * abs(float(ce)) + 2 * (n_add(V) + 70) * U
+
+
+@pytest.mark.parametrize("rows", [1, 700, 1023, 1024, 1025, 3000])
+@pytest.mark.parametrize("V", [129, 17001])
+def test_means_over_few_and_many_rows(rows, V):
+    """The rows that count are counted in two ways, and dealt among teams from some number on: the mean, its gradient and the
+    rows that hold nothing, with labels that count in runs, at random, hardly any, and all."""
+    from speech_to_text_amd import distillation_loss_and_grad, token_logprobs
+    rng = np.random.default_rng(rows + V)
+    z = randn((1, V), torch.bfloat16, V, scale=2.0).to(DEV).repeat(rows, 1)
+    for kind in ("all", "runs", "random", "few"):
+        y = rng.integers(0, V, rows)
+        keep = {"all": np.ones(rows, bool), "runs": np.arange(rows) % 97 < 40, "random": rng.random(rows) < 0.6,
+                "few": np.arange(rows) == rows // 2}[kind]
+        y[~keep] = -100
+        yt = torch.from_numpy(y).to(DEV)
+        ids = torch.full((rows, 2), 5, device=DEV)
+        t = torch.zeros(rows, 2, device=DEV)
+        want, grad, size = O.distillation(np64(z[:1]), np.array([7]), np.array([[5, 5]]), np.zeros((1, 2)), 2.0, 0.5)
+        lp = O.log_softmax(np64(z[:1]))[0]
+        n = keep.sum()
+        each = np.where(keep, want[0] + 0.5 * lp[7] - 0.5 * lp[np.maximum(y, 0)], 0.0)
+        loss, g = distillation_loss_and_grad(z, yt, ids, t, temperature=2.0)
+        tol = (n_add(V) + 400) * 20 * U * np.abs(each).max()
+        assert abs(float(loss) - each.sum() / max(n, 1)) <= tol
+        off = g.float()
+        assert (off[torch.from_numpy(~keep).to(DEV)] == 0).all()
+        if n == 0:
+            continue
+        r = int(np.flatnonzero(keep)[-1])
+        w = grad[0].copy()
+        w[7] += 0.5
+        w[y[r]] -= 0.5
+        sz = size[0].copy()
+        sz[y[r]] += 1.0
+        check_grad(g[r], (w / n)[None], (sz / n)[None], torch.bfloat16, V)
+        s = token_logprobs(z, yt, top_k=3, entropy=True)
+        assert np.abs(np64(s.logprobs) - np.where(keep, lp[np.maximum(y, 0)], 0.0)).max() <= (n_add(V) + 70 + 80) * U
+        assert ((s.entropy == 0).cpu().numpy() == ~keep).all()
+        assert ((s.top_ids[:, 0] == -1).cpu().numpy() == ~keep).all() and len(s.top_ids[torch.from_numpy(keep).to(DEV)].unique(dim=0)) == 1
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_wide_vocabulary_many_rows(dtype):
+    """Rows of several segments, more than the chip's teams: ragged labels, scores and gradients."""
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    rows, V, K = 700, 70001, 6
+    z = randn((5, V), TYPES[dtype], 3).to(DEV)
+    pick = torch.arange(rows, device=DEV) % 5
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(1)).to(DEV)
+    y[torch.arange(rows, device=DEV) % 7 > 3] = -100
+    x = z[pick]
+    rng = np.random.default_rng(1)
+    ids5, t5 = rng.integers(0, V, (5, K)), rng.standard_normal((5, K)).astype(np.float32)
+    ids, t = torch.from_numpy(ids5).to(DEV)[pick], torch.from_numpy(t5).to(DEV)[pick]
+    s = token_logprobs(x, y, top_k=K, entropy=True)
+    _, h, top, _ = O.token_logprobs(np64(z), None, K)
+    lp = O.log_softmax(np64(z))
+    live, p5, yn = (y >= 0).cpu().numpy(), pick.cpu().numpy(), y.cpu().numpy()
+    same(np64(s.logprobs), np.where(live, lp[p5, np.maximum(yn, 0)], 0.0), np.full(rows, (n_add(V) + 70 + 80) * U), "logprobs")
+    same(np64(s.entropy), np.where(live, h[p5], 0.0), np.full(rows, (n_add(V) + 70) * (1 + np.log2(V + 1)) * U), "entropy")
+    assert np.array_equal(s.top_ids.cpu().numpy(), np.where(live[:, None], top[p5], -1))
+    x.requires_grad_()
+    for red, f in (("sum", 1.0), ("mean", 1.0 / live.sum())):
+        loss = distillation_loss(x, y, ids, t, temperature=3.0, alpha=0.7, weight=0.5, reduction=red)
+        g, = torch.autograd.grad(loss, x)
+        assert (g[~torch.from_numpy(live).to(DEV)] == 0).all()
+        rs = [int(r) for r in np.flatnonzero(live)[[0, 1, 7, -1]]]
+        want, grad, size = O.distillation(np64(x[rs]), yn[rs], ids5[p5[rs]], t5[p5[rs]], 3.0, 0.7)
+        check_grad(g[rs], grad * f * 0.5, size * f * 0.5, TYPES[dtype], V)
+        every, _, _ = O.distillation(np64(z), np.zeros(5, np.int64), ids5, t5, 3.0, 0.7)
+        total = sum(every[p5[r]] + 0.3 * lp[p5[r], 0] - 0.3 * lp[p5[r], yn[r]] for r in np.flatnonzero(live)) * f * 0.5
+        assert abs(float(loss.detach()) - total) <= (n_add(V) + 400) * 20 * U * abs(total)
