@@ -14,8 +14,6 @@ constexpr int kMaxWaves = 8, kMaxVpt = 16;       // the largest team: waves, and
 constexpr bool kScoreAhead(bool top) { return !top; }
 constexpr bool kDistillAhead = true;
 constexpr int kWavesPerSimd(int vpt, bool ahead) { return vpt >= 16 && ahead ? 2 : 4; }
-constexpr int kCand = 512;                       // alternatives' candidates a team sorts at once
-constexpr int kStage = 64;                       // ... of which a wave may bring this many
 constexpr int kGroups = 256;                     // groups of elements whose maxima bound the alternatives
 constexpr int kMaxSegs = 64;                     // segments of a row: one lane each when they are joined
 constexpr float kLn2 = 0.693147180559945309f;

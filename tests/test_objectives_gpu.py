@@ -601,3 +601,60 @@ def test_wide_vocabulary_many_rows(dtype):
         every, _, _ = O.distillation(np64(z), np.zeros(5, np.int64), ids5, t5, 3.0, 0.7)
         total = sum(every[p5[r]] + 0.3 * lp[p5[r], 0] - 0.3 * lp[p5[r], yn[r]] for r in np.flatnonzero(live)) * f * 0.5
         assert abs(float(loss.detach()) - total) <= (n_add(V) + 400) * 20 * U * abs(total)
+
+
+def hard_rows(V, dtype, seed):
+    """Rows whose alternatives are not few elements above a bound: sorted, equal, masked, NaN in places, few distinct values."""
+    g = torch.Generator().manual_seed(seed)
+    rows = {}
+    rows["rising"] = torch.linspace(-8, 12, V)
+    rows["falling"] = torch.linspace(12, -8, V)
+    rows["equal"] = torch.full((V,), 1.5)
+    rows["equal below 0"] = torch.full((V,), -1.5)
+    zeros = torch.zeros(V)
+    zeros[torch.arange(V) % 3 == 1] = -0.0
+    rows["zeros of both signs"] = zeros
+    few = torch.full((V,), -float("inf"))
+    few[torch.randperm(V, generator=g)[: 8]] = torch.randn(min(8, V), generator=g)
+    rows["masked to 8"] = few
+    run = torch.full((V,), -float("inf"))
+    run[V // 3 : V // 3 + 500] = torch.randn(len(run[V // 3 : V // 3 + 500]), generator=g)
+    rows["masked to a run"] = run
+    rows["two values"] = (torch.rand(V, generator=g) < 0.5).float()
+    rows["quarters"] = (torch.randn(V, generator=g) * 4).round() / 4 - 3
+    block = torch.randn(V, generator=g)
+    block[V // 2 : V // 2 + 90] += 20
+    rows["a high block"] = block
+    lowest = torch.full((V,), torch.finfo(dtype).min)
+    lowest[torch.randperm(V, generator=g)[: 3]] = 2.0
+    rows["lowest value but 3"] = lowest
+    for name, n in (("a few NaN", 3), ("many NaN", 200)):
+        nan = torch.randn(V, generator=g)
+        nan[torch.randperm(V, generator=g)[:n]] = float("nan")
+        rows[name] = nan
+    nan = torch.full((V,), -float("inf"))
+    nan[-1] = float("nan")
+    rows["NaN behind -inf"] = nan
+    inf = torch.randn(V, generator=g)
+    inf[torch.randperm(V, generator=g)[: 100]] = float("inf")
+    rows["many inf"] = inf
+    rows["nothing but -inf"] = torch.full((V,), -float("inf"))
+    return rows
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V", [70, 401, 2000, 4099, 10007, 32001, 50021, 200019])
+def test_alternatives_of_hard_rows(V, dtype):
+    """The ids are exact whatever the row: value falling, NaN first, equal values by index.  Every row at two alignments."""
+    from speech_to_text_amd import token_logprobs
+
+    rows = hard_rows(V, TYPES[dtype], V)
+    z = torch.stack(list(rows.values())).to(TYPES[dtype])
+    store = torch.zeros((len(rows), V + 3), dtype=TYPES[dtype], device=DEV)
+    store[:, 2 : V + 2] = z.to(DEV)
+    for k in (1, 7, 16, 64):
+        want = [O.alternatives(np64(row), k) for row in z]
+        for x in (z.to(DEV), store[:, 2 : V + 2]):
+            got = token_logprobs(x, top_k=k).top_ids.cpu().numpy()
+            for r, name in enumerate(rows):
+                assert np.array_equal(got[r], want[r]), (name, k)
