@@ -306,11 +306,13 @@ int sttfe_pitch_shift(float* pcm, const int64_t* offsets, const int32_t* lengths
  *   labels       : device int64 [outer * inner]; rows with label == ignore_index hold no token: they are not read, their
  *                  results are 0 (ids -1, top log probabilities -inf) and their gradient is 0.  Any other label outside
  *                  [0, vocab) cannot be reported without synchronising: the row's results and its gradient are NaN.
- *   temperature  : > 0; the softmax is that of logits / temperature.
- *   stats        : device float32 [outer * inner][4], written by the forward call for the gradient call (NULL: not wanted).
+ *   temperature  : in [1e-6, 1e6]; the softmax is that of logits / temperature.
+ *   stats        : device float32 [outer * inner][4], 16-byte aligned as the workspace is, written by the forward call for the
+ *                  gradient call (NULL: not wanted).
  * A row that holds NaN or +inf, or nothing but -inf, has no softmax: its results are NaN, as torch.log_softmax's are
  * (alternatives: NaN counts as the largest value).  A -inf logit among others has probability 0 and adds nothing.
- * All sums are float32 or wider and in a fixed order: the same inputs give the same bits.
+ * All sums are float32 or wider and in a fixed order, which the alignment of a row (address modulo 16) decides with its
+ * length: the same inputs at the same alignment give the same bits, in whatever call.
  */
 #define STTFE_DTYPE_F32 0
 #define STTFE_DTYPE_F16 1

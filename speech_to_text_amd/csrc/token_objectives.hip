@@ -10,7 +10,6 @@
 namespace sttfe {
 namespace {
 
-
 // Rows that count, by one team.
 constexpr int kRowsThreads = 1024;
 __device__ int count_rows(const int64_t* __restrict__ labels, int64_t ignore, int64_t rows, int* part) {
@@ -103,7 +102,9 @@ int check_rows(const void* logits, int dtype, int64_t outer, int64_t inner, int6
     return STTFE_OK;
 }
 
-bool positive(float x) { return x > 0.f && x <= 3.4e38f; }
+// c = log2(e) / T and T^2 stay far inside float's range.
+bool temperature_ok(float t) { return t >= 1e-6f && t <= 1e6f; }
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }       // read and written as float4
 
 }  // namespace
 }  // namespace sttfe
@@ -131,10 +132,11 @@ extern "C" int sttfe_token_logprobs(const void* logits, int dtype, int64_t outer
                                     int64_t* top_ids, float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream_) {
     int rc = check_rows(logits, dtype, outer, inner, stride_outer, stride_inner, vocab);
     if (rc != STTFE_OK) return rc;
-    if (!positive(temperature) || top_k < 0 || top_k > STTFE_MAX_TOP || top_k > vocab) return STTFE_E_INVALID_ARG;
+    if (!temperature_ok(temperature) || top_k < 0 || top_k > STTFE_MAX_TOP || top_k > vocab) return STTFE_E_INVALID_ARG;
     const int64_t n = outer * inner;
     if (n == 0) return STTFE_OK;
     if ((logprobs && !labels) || (top_k > 0 && (!top_ids || !top_logprobs))) return STTFE_E_INVALID_ARG;
+    if (!aligned16(stats) || !aligned16(workspace)) return STTFE_E_INVALID_ARG;
     size_t need = 0;
     rc = sttfe_token_logprobs_workspace_bytes(n, vocab, dtype, top_k, &need);
     if (rc != STTFE_OK) return rc;
@@ -163,10 +165,10 @@ extern "C" int sttfe_token_logprobs_grad(const void* logits, int dtype, int64_t 
                                          int top_k, const int64_t* top_ids, const float* g_top, void* grad, void* stream_) {
     int rc = check_rows(logits, dtype, outer, inner, stride_outer, stride_inner, vocab);
     if (rc != STTFE_OK) return rc;
-    if (!positive(temperature) || top_k < 0 || top_k > STTFE_MAX_TOP || top_k > vocab) return STTFE_E_INVALID_ARG;
+    if (!temperature_ok(temperature) || top_k < 0 || top_k > STTFE_MAX_TOP || top_k > vocab) return STTFE_E_INVALID_ARG;
     const int64_t n = outer * inner;
     if (n == 0) return STTFE_OK;
-    if (!stats || !grad || (g_logprobs && !labels) || (g_top && (top_k == 0 || !top_ids))) return STTFE_E_INVALID_ARG;
+    if (!stats || !aligned16(stats) || !grad || (g_logprobs && !labels) || (g_top && (top_k == 0 || !top_ids))) return STTFE_E_INVALID_ARG;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = grad_plan(vocab, dtype);
@@ -183,7 +185,7 @@ extern "C" int sttfe_token_logprobs_grad(const void* logits, int dtype, int64_t 
 }
 
 static int check_distill(const int64_t* labels, const int64_t* ids, const float* teacher, int K, float tau, float alpha) {
-    if (!labels || !ids || !teacher || K < 1 || K > STTFE_MAX_TOP || !positive(tau) || !(alpha >= 0.f && alpha <= 1.f))
+    if (!labels || !ids || !teacher || K < 1 || K > STTFE_MAX_TOP || !temperature_ok(tau) || !(alpha >= 0.f && alpha <= 1.f))
         return STTFE_E_INVALID_ARG;
     return STTFE_OK;
 }
@@ -209,7 +211,7 @@ extern "C" int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, 
     if (n > 0) {
         rc = check_distill(labels, teacher_ids, teacher_logits, teacher_k, temperature, alpha);
         if (rc != STTFE_OK) return rc;
-        if (!losses) return STTFE_E_INVALID_ARG;
+        if (!losses || !aligned16(stats) || !aligned16(workspace)) return STTFE_E_INVALID_ARG;
     }
     if (n == 0 && reduction == STTFE_REDUCE_NONE) return STTFE_OK;
     size_t need = 0;
@@ -271,7 +273,7 @@ extern "C" int sttfe_distill_grad(const void* logits, int dtype, int64_t outer, 
     if (n == 0) return STTFE_OK;
     rc = check_distill(labels, teacher_ids, teacher_logits, teacher_k, temperature, alpha);
     if (rc != STTFE_OK) return rc;
-    if (!stats || !grad) return STTFE_E_INVALID_ARG;
+    if (!stats || !aligned16(stats) || !grad) return STTFE_E_INVALID_ARG;
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = grad_plan(vocab, dtype);

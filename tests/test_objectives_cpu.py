@@ -193,3 +193,26 @@ def test_teacher_refusals(tmp_path):
         FeatureCacheWriter(str(tmp_path), "whisper", 80, teacher_top=65)
     assert w.shards == []                      # a refused batch leaves nothing behind
     w.close()
+
+
+def test_c_abi_refuses_unaligned_statistics_and_temperatures_out_of_range():
+    L = _lib.lib()
+    p, odd = ctypes.c_void_p(64), ctypes.c_void_p(72)      # never dereferenced: every call below is refused
+
+    def score(stats=None, ws=None, temp=1.0):
+        return L.sttfe_token_logprobs(p, 0, 2, 3, 33, 11, 11, p, -100, temp, 0, p, None, stats, None, None, ws, 0, None)
+
+    def grad(stats=p, temp=1.0):
+        return L.sttfe_token_logprobs_grad(p, 0, 2, 3, 33, 11, 11, p, -100, temp, stats, p, None, 0, None, None, p, None)
+
+    def distill(stats=None, ws=None, temp=1.0):
+        return L.sttfe_distill_loss(p, 2, 2, 3, 33, 11, 11, p, -100, p, p, 4, temp, 0.5, 1.0, 2, p, p, p, stats, None, ws, 0, None)
+
+    def distill_grad(stats=p, temp=1.0):
+        return L.sttfe_distill_grad(p, 2, 2, 3, 33, 11, 11, p, -100, p, p, 4, temp, 0.5, stats, None, None, None, p, None)
+
+    for call in (score, grad, distill, distill_grad):
+        assert call(stats=odd) == -1
+        for temp in (1e-7, 1e7, -1.0, float("nan"), float("inf")):
+            assert call(temp=temp) == -1
+    assert score(ws=odd) == -1 and distill(ws=odd) == -1

@@ -658,3 +658,75 @@ def test_alternatives_of_hard_rows(V, dtype):
             got = token_logprobs(x, top_k=k).top_ids.cpu().numpy()
             for r, name in enumerate(rows):
                 assert np.array_equal(got[r], want[r]), (name, k)
+
+
+@pytest.mark.parametrize("T", [1e-3, 1e3])
+@pytest.mark.parametrize("V", [401, 32001])
+def test_extreme_temperatures(V, T):
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    z = randn((5, V), torch.float32, V, offset=40.0)
+    y = torch.randint(0, V, (5,), generator=torch.Generator().manual_seed(V))
+    check_scores(token_logprobs(z.to(DEV), y.to(DEV), top_k=9, entropy=True, temperature=T), z, y, 9, T)
+    ids, teacher = teacher_rows(5, V, 6, V)
+    want, grad, size = O.distillation(np64(z), y.numpy(), ids.numpy(), teacher.numpy(), T, 0.5)
+    x = z.to(DEV).requires_grad_()
+    each = distillation_loss(x, y.to(DEV), ids.to(DEV), teacher.to(DEV), temperature=T, reduction="none")
+    check_losses(np64(each), want, np64(z), y.numpy(), ids.numpy(), teacher.numpy(), T, 0.5)
+    d, = torch.autograd.grad(each.sum(), x)
+    check_grad(d, grad, size, torch.float32, V)
+
+
+@pytest.mark.parametrize("V", [2000, 9001, 66001])
+def test_more_rows_than_are_dealt_at_once(V):
+    """Rows far apart in a call of 20000 (several rounds of dealing them out, many of them ignored) have the bits that they have
+    alone, read from the same place: the alignment of a row decides the order of its sums."""
+    from speech_to_text_amd import distillation_loss, distillation_loss_and_grad, token_logprobs
+    n = 20000
+    g = torch.Generator(device=DEV).manual_seed(V)
+    z = torch.empty((n, V), dtype=torch.bfloat16, device=DEV).normal_(0, 2.5, generator=g)
+    y = torch.randint(0, V, (n,), generator=g, device=DEV)
+    y[torch.rand(n, generator=g, device=DEV) < 0.3] = -100
+    y[5000:9000] = -100
+    ids = torch.randint(0, V, (n, 4), generator=g, device=DEV)
+    t = torch.randn((n, 4), generator=g, device=DEV)
+    some = (0, 1, 255, 256, 1023, 4999, 5000, 8191, 8192, 9000, 12345, 16383, 16384, 16385, 19998, 19999)
+    for k in (0, 5):
+        got = token_logprobs(z, y, top_k=k, entropy=True)
+        for r in some:
+            alone = token_logprobs(z[r : r + 1], y[r : r + 1], top_k=k, entropy=True)
+            assert all(torch.equal(a[r : r + 1], b) for a, b in zip(got, alone) if a is not None), r
+        assert bool((got.logprobs[y == -100] == 0).all()) and bool((got.entropy[y == -100] == 0).all())
+        assert bool((got.logprobs[y != -100] < 0).all())
+    each = distillation_loss(z, y, ids, t, temperature=2.0, reduction="none")
+    loss, grad = distillation_loss_and_grad(z, y, ids, t, temperature=2.0, reduction="sum")
+    for r in some:
+        one = tuple(v[r : r + 1] for v in (z, y, ids, t))
+        assert torch.equal(each[r : r + 1], distillation_loss(*one, temperature=2.0, reduction="none")), r
+        assert torch.equal(grad[r : r + 1], distillation_loss_and_grad(*one, temperature=2.0, reduction="sum")[1]), r
+    assert bool((grad[y == -100] == 0).all()) and bool((grad.abs().amax(1)[y != -100] > 0).all())
+    total = float(each.double().sum())
+    assert abs(float(loss) - total) <= 2 * U * abs(total)
+
+
+@pytest.mark.parametrize("V", [5003, 70001])
+def test_two_streams_at_once(V):
+    """Calls on two streams that run side by side share nothing."""
+    from speech_to_text_amd import distillation_loss_and_grad, token_logprobs
+    sets, want = [], []
+    for s in range(2):
+        z = randn((300, V), torch.bfloat16, s).to(DEV)
+        y = torch.randint(0, V, (300,), generator=torch.Generator().manual_seed(s)).to(DEV)
+        sets.append((z, y, *(v.to(DEV) for v in teacher_rows(300, V, 8, s))))
+        want.append((token_logprobs(z, y, top_k=7, entropy=True), distillation_loss_and_grad(*sets[s], temperature=2.0)))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for s in range(2):
+            with torch.cuda.stream(streams[s]):
+                z, y = sets[s][:2]
+                got[s].append((token_logprobs(z, y, top_k=7, entropy=True), distillation_loss_and_grad(*sets[s], temperature=2.0)))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for scores, (loss, grad) in got[s]:
+            assert all(torch.equal(a, b) for a, b in zip(scores, want[s][0]))
+            assert torch.equal(loss, want[s][1][0]) and torch.equal(grad, want[s][1][1])
