@@ -30,10 +30,11 @@ struct Rows {                      // row r = (r / inner, r % inner)
     int vocab, segs, seg_len;      // a row is cut into segs segments of seg_len elements (the last may be shorter)
 };
 
+constexpr double kClimb = 4.0;     // bits by which an element may exceed the reference of a wave's sums
 struct Score {
     const int64_t* labels;
     int64_t ignore;
-    float c, inv_t;
+    float c, inv_t, climb;                       // log2(e) / T, 1 / T; kClimb / c
     int top_k;
     float *logprobs, *entropy, *stats;
     int64_t* top_ids;
@@ -64,7 +65,7 @@ struct Distill {
     const float* logits;
     int64_t ignore;
     int K;
-    float tau, inv_tau, alpha, c, c1;            // c: of the first softmax, c1: of the second (or of the only one)
+    float tau, inv_tau, alpha, c, c1, climb;     // c: of the first softmax, c1: of the second (or of the only one)
     bool teacher, label;                         // which terms there are
 };
 

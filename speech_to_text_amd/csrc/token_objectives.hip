@@ -85,8 +85,9 @@ int dealt_teams(const Plan& plan, int64_t n, bool ahead) {
 }
 
 Distill distill_args(const int64_t* labels, int64_t ignore, const int64_t* ids, const float* teacher, int K, float tau, float alpha) {
-    Distill a{labels, ids, teacher, ignore, K, tau, (float)(1.0 / (double)tau), alpha, 0.f, (float)kLog2e, alpha != 0.f, alpha != 1.f};
+    Distill a{labels, ids, teacher, ignore, K, tau, (float)(1.0 / (double)tau), alpha, 0.f, (float)kLog2e, 0.f, alpha != 0.f, alpha != 1.f};
     a.c = a.teacher ? (float)(kLog2e / (double)tau) : (float)kLog2e;
+    a.climb = (float)(kClimb / (double)(a.label && a.c1 > a.c ? a.c1 : a.c));
     return a;
 }
 Mode distill_mode(const Distill& a) {
@@ -148,8 +149,8 @@ extern "C" int sttfe_token_logprobs(const void* logits, int dtype, int64_t outer
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     float4* parts = static_cast<float4*>(workspace);
     const int teams = dealt_teams(plan, n, kScoreAhead(top_k > 0));
-    const Score a{labels, ignore_index, (float)(kLog2e / (double)temperature), (float)(1.0 / (double)temperature), top_k, logprobs, entropy,
-                  stats, top_ids, top_logprobs, parts, reinterpret_cast<uint64_t*>(parts + (plan.segs > 1 ? n * plan.segs : 0)), (uint32_t)n, teams > 0};
+    const Score a{labels, ignore_index, (float)(kLog2e / (double)temperature), (float)(1.0 / (double)temperature),
+                  (float)(kClimb / kLog2e * (double)temperature), top_k, logprobs, entropy, stats, top_ids, top_logprobs, parts, reinterpret_cast<uint64_t*>(parts + (plan.segs > 1 ? n * plan.segs : 0)), (uint32_t)n, teams > 0};
     {
         ScopedTiming t(kTimeTokenLogprobs, stream);
         STTFE_BY_DTYPE(dtype, Launch<T>::score(plan, rows, a, (unsigned)(teams ? teams : n * plan.segs), entropy || stats, stream));

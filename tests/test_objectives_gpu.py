@@ -730,3 +730,119 @@ def test_two_streams_at_once(V):
         for scores, (loss, grad) in got[s]:
             assert all(torch.equal(a, b) for a, b in zip(scores, want[s][0]))
             assert torch.equal(loss, want[s][1][0]) and torch.equal(grad, want[s][1][1])
+
+
+def confident_rows(V, dtype, seed):
+    """Rows in which one token (or two, or a stair of them) stands `gap` nats above all others, anywhere in the row, as a model
+    that is sure of its transcript gives them; and rows of one large negative value.  -> rows, index of each row's largest."""
+    g = torch.Generator().manual_seed(seed)
+    rng = np.random.default_rng(seed)
+    rows = []
+    for n, gap in enumerate((0.5, 1.5, 2.5, 3.5, 5.0, 8.0, 12.0, 16.0, 20.0, 25.0, 30.0, 40.0)):
+        for at in {0, V - 1, V // 2 + n, *(int(v) for v in rng.integers(0, V, 2))}:
+            z = torch.randn(V, generator=g) + (3.0 if n % 2 else -60.0)
+            z[at] = z.max() + gap
+            rows.append(z)
+    for gap in (10.0, 25.0):
+        z = torch.randn(V, generator=g)
+        z[[V // 3, 2 * V // 3]] = float(z.max()) + gap
+        rows.append(z)
+    z = torch.randn(V, generator=g)
+    stair = torch.arange(7, V, max(1, V // 23))
+    z[stair] = 5.0 + 2.0 * torch.arange(len(stair)).float()                # rises by less than is climbed at once, and goes on
+    rows.append(z)
+    z = torch.full((V,), -float("inf"))
+    z[V // 5], z[V - V // 5 - 1] = 1.0, 28.0
+    rows.append(z)
+    for low in (-1e4, -3e4, -1e9 if dtype != torch.float16 else -6e4):
+        rows.append(torch.full((V,), low))
+        z = torch.full((V,), low)
+        z[rng.integers(0, V, 3)] = torch.tensor([0.0, -1.0, 24.0])
+        rows.append(z)
+    z = torch.stack(rows).to(dtype)
+    return z, z.float().argmax(1)
+
+
+def sums_of(z, T):
+    """What the bars of confident rows need of a row, in float64: log probabilities, ln S, relative error of S, A, A2, eps."""
+    lp = O.log_softmax(z, T)
+    p, top = np.exp(lp), lp.max(-1)
+    a = (top[:, None] - np.where(np.isfinite(lp), lp, top[:, None])) / np.log(2)      # distance from the largest, in bits
+    A, A2 = (p * a).sum(-1), (p * a * a).sum(-1)
+    first = lp.argmax(-1)
+    rest = p * (np.arange(z.shape[1]) != first[:, None])
+    eps, eps_w = rest.sum(-1), (rest * (a + 4.1)).sum(-1)
+    rel = (4.3 * A + 22) * U + np.minimum(n_add(z.shape[1]) * U, eps)
+    return lp, -top, rel, A, A2, eps_w, a
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("V, T", [(401, 1.0), (2000, 1.0), (10007, 1.0), (10007, 0.6), (32001, 1.0), (50021, 1.0), (50021, 2.5),
+                                  (51865, 1.0), (200019, 1.0)])
+def test_confident_rows(V, T, dtype):
+    """Sure tokens keep the precision of a softmax taken against the row's maximum: no log probability above 0, no entropy below 0,
+    and bars without the slack of a flat row.
+
+    With a_j the distance of element j from the row's largest in bits, all powers of two are taken within 4.1 bits of the
+    maximum, so a term of S is off by (4.3 a_j + 14) u (rounded exponents 2.8 a_j + 5.7, three exponentials 6, products 2, steps
+    from one reference to a higher one 1.5 a_j; the square of a power, for a second softmax, 8 more), and adding errs by n_add u at
+    most, and by no more than what is added: eps = the mass outside the largest element.
+      |dS / S| <= rel = (4.3 A + 22) u + min(n_add u, eps),  A = sum p a
+      |d lp| <= rel + (2 + 4 ln S + 3 |lp|) u
+      |d W| <= (4.3 A2 + 19 A + 17) u + min(n_add (A + 4.1) u, eps_w), A2 = sum p a^2, eps_w = sum over the others p (a + 4.1)
+      |d H| <= ln 2 (|d W| + A rel + 3 A u) + rel + (4 ln S + 2 H) u
+      |d p_j| <= p_j (rel + (10 + 4 ln S + 2.8 a_j) u), or 2^-126 where p_j is below that: v_exp_f32 flushes its result, and the
+    flushed p_j is then multiplied by 1 / T (by alpha tau and 1 - alpha), so that 2^-126 is, too."""
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    t = TYPES[dtype]
+    z, at = confident_rows(V, t, V)
+    n = len(z)
+    other = torch.randint(0, V, (n,), generator=torch.Generator().manual_seed(V))
+    store = torch.zeros((n, V + 3), dtype=t, device=DEV)
+    store[:, 1 : V + 1] = z.to(DEV)
+    lp, ln_s, rel, A, A2, eps_w, a = sums_of(np64(z), T)
+    p = np.exp(lp)
+    h = -np.where(p > 0, p * np.where(p > 0, lp, 0.0), 0.0).sum(-1)
+    dw = (4.3 * A2 + 19 * A + 17) * U + np.minimum(n_add(V) * (A + 4.1) * U, eps_w)
+    bar_h = np.log(2) * (dw + A * rel + 3 * A * U) + rel + (4 * ln_s + 2 * h) * U
+    rows = np.arange(n)
+    for y in (at, other):
+        want = lp[rows, y.numpy()]
+        bar = rel + (2 + 4 * ln_s + 3 * np.abs(want)) * U
+        for x in (z.to(DEV), store[:, 1 : V + 1]):
+            for k in (0, 4):
+                got = token_logprobs(x, y.to(DEV), top_k=k, entropy=True, temperature=T)
+                same(np64(got.logprobs), want, bar, "logprobs")
+                same(np64(got.entropy), h, bar_h, "entropy")
+                assert not (got.logprobs > 0).any() and not (got.entropy < 0).any()
+                if k:
+                    assert np.array_equal(got.top_ids[:, 0].cpu().numpy(), at.numpy()) and not (got.top_logprobs > 0).any()
+                    top = np.take_along_axis(lp, got.top_ids.cpu().numpy(), 1)
+                    same(np64(got.top_logprobs), top, rel[:, None] + (2 + 4 * ln_s[:, None] + 3 * np.abs(top)) * U, "top_logprobs")
+    # gradient of the sure token's log probability: p_j, and 1 - p of its own
+    info, tiny = torch.finfo(t), 2.0 ** -25 if dtype == "fp16" else 2.0 ** -126
+    x = z.to(DEV).requires_grad_()
+    d, = torch.autograd.grad(token_logprobs(x, at.to(DEV), temperature=T).logprobs.sum(), x)
+    dp = p * (rel[:, None] + (10 + 4 * ln_s[:, None] + 2.8 * a) * U)
+    one = np.arange(V) == at.numpy()[:, None]
+    want = (one - p) / T
+    same(np64(d), want, dp / T + (info.eps / 2 + 2 * U) * np.abs(want) * (1 + 2 ** -10) + tiny + 2.0 ** -126 / T, "grad")
+    # distillation with the sure token as the teacher's only entry and as the label
+    ids, teacher, alpha = at[:, None].to(DEV), torch.zeros(n, 1, device=DEV), 0.5
+    for tau in (1.0, 2.0, 3.0):
+        lpt, ln_t, rel_t, _, _, _, a_t = sums_of(np64(z), tau)
+        lp1, ln_1, rel_1, _, _, _, a_1 = sums_of(np64(z), 1.0)
+        want = alpha * tau ** 2 * -lpt[rows, at] - (1 - alpha) * lp1[rows, at]
+        bar = (alpha * tau ** 2 * (rel_t + (2 + 4 * ln_t) * U) + (1 - alpha) * (rel_1 + (2 + 4 * ln_1) * U) + 6 * U * np.abs(want))
+        each = distillation_loss(x, at.to(DEV), ids, teacher, temperature=tau, alpha=alpha, reduction="none")
+        same(np64(each), want, bar, "loss")
+        assert not (each < 0).any()
+        pt, p1 = np.exp(lpt), np.exp(lp1)
+        grad = alpha * tau * (pt - one) + (1 - alpha) * (p1 - one)
+        dg = (alpha * tau * pt * (rel_t[:, None] + (12 + 4 * ln_t[:, None] + 2.8 * a_t) * U)
+              + (1 - alpha) * p1 * (rel_1[:, None] + (12 + 4 * ln_1[:, None] + 2.8 * a_1) * U) + 3 * U * (alpha * tau + 1 - alpha) * one)
+        tol = dg + (info.eps / 2 + 2 * U) * np.abs(grad) * (1 + 2 ** -10) + tiny + 2.0 ** -126 * (alpha * tau + 1 - alpha)
+        d, = torch.autograd.grad(each, x, torch.ones(n, device=DEV))
+        same(np64(d), grad, tol, "grad")
+        d, = torch.autograd.grad(distillation_loss(x, at.to(DEV), ids, teacher, temperature=tau, alpha=alpha, reduction="sum"), x)
+        same(np64(d), grad, tol, "grad of the sum")
