@@ -846,3 +846,27 @@ def test_confident_rows(V, T, dtype):
         same(np64(d), grad, tol, "grad")
         d, = torch.autograd.grad(distillation_loss(x, at.to(DEV), ids, teacher, temperature=tau, alpha=alpha, reduction="sum"), x)
         same(np64(d), grad, tol, "grad of the sum")
+
+
+@pytest.mark.parametrize("alpha", [0.0, 0.5, 1.0])
+@pytest.mark.parametrize("V", [300, 10007, 140001])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_outside_the_vocabulary_is_nan_whatever_the_terms(dtype, V, alpha):
+    """A label or an id outside the vocabulary makes loss and gradient of its row NaN: with and without the teacher's term or the
+    label's, with entries that are all outside (none is kept), and beside a row that keeps none and is sound."""
+    from speech_to_text_amd import distillation_loss, distillation_loss_and_grad
+    z = randn((8, V), TYPES[dtype], V)
+    y = torch.tensor([V, 5, 7, -100, -1, 2, 2 ** 40, 3])
+    ids = torch.tensor([[1, 2], [V, V + 3], [V, -1], [V, V], [-1, -1], [-1, -1], [4, 4], [5, V]])
+    bad = torch.tensor([True, True, True, False, True, False, True, True])
+    teacher = torch.zeros(8, 2)
+    x = z.to(DEV).requires_grad_()
+    args = (y.to(DEV), ids.to(DEV), teacher.to(DEV))
+    for tau in (1.0, 2.0, 3.0):
+        each = distillation_loss(x, *args, temperature=tau, alpha=alpha, reduction="none")
+        d, = torch.autograd.grad(each, x, torch.ones(8, device=DEV))
+        s, = torch.autograd.grad(distillation_loss(x, *args, temperature=tau, alpha=alpha, reduction="sum"), x)
+        total, m = distillation_loss_and_grad(x, *args, temperature=tau, alpha=alpha)
+        assert torch.equal(each.detach().isnan().cpu(), bad) and bool(total.isnan())
+        for g in (d, s, m):
+            assert torch.equal(g.isnan().all(1).cpu(), bad) and not g[~bad.to(DEV)].isnan().any() and bool((g[3] == 0).all())
