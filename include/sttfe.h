@@ -305,7 +305,9 @@ int sttfe_pitch_shift(float* pcm, const int64_t* offsets, const int32_t* lengths
  *                  alignment of one element only.  At most STTFE_MAX_ROWS rows, vocab in [1, STTFE_MAX_VOCAB].
  *   labels       : device int64 [outer * inner]; rows with label == ignore_index hold no token: they are not read, their
  *                  results are 0 (ids -1, top log probabilities -inf) and their gradient is 0.  Any other label outside
- *                  [0, vocab) cannot be reported without synchronising: the row's results and its gradient are NaN.
+ *                  [0, vocab) cannot be reported without synchronising: what is asked of the label is NaN (its log
+ *                  probability and the gradient that comes with it, a distillation's loss and gradient); entropy and
+ *                  alternatives are those of the row, whatever its label, and so are the gradients of those alone.
  *   temperature  : in [1e-6, 1e6]; the softmax is that of logits / temperature.
  *   stats        : device float32 [outer * inner][4], 16-byte aligned as the workspace is, written by the forward call for the
  *                  gradient call (NULL: not wanted).

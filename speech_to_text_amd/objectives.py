@@ -175,7 +175,8 @@ def token_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
     alternatives, no gradient.  ``top_k`` <= 64: the largest logits in falling order, equal ones by index.
 
     ``logprobs``, ``entropy`` and ``top_logprobs`` are differentiable in the logits (once).  A label outside the vocabulary
-    makes its position NaN: it cannot be reported without a synchronisation.
+    makes its log probability NaN, and the gradient that comes with it: it cannot be reported without a synchronisation.
+    Entropy and alternatives do not depend on the label.
     """
     what = "token_logprobs"
     rows = _rows(logits, what)

@@ -870,3 +870,22 @@ def test_outside_the_vocabulary_is_nan_whatever_the_terms(dtype, V, alpha):
         assert torch.equal(each.detach().isnan().cpu(), bad) and bool(total.isnan())
         for g in (d, s, m):
             assert torch.equal(g.isnan().all(1).cpu(), bad) and not g[~bad.to(DEV)].isnan().any() and bool((g[3] == 0).all())
+
+
+@pytest.mark.parametrize("V", [300, 50021, 140001])
+def test_entropy_and_alternatives_do_not_depend_on_the_label(V):
+    """A label outside the vocabulary is NaN where it is asked for and nowhere else; a gradient without its log probability is that
+    of the same row with any other label."""
+    from speech_to_text_amd import token_logprobs
+    z = randn((4, V), torch.bfloat16, V).to(DEV)
+    bad, good = torch.tensor([V, -1, 2 ** 40, 3], device=DEV), torch.tensor([0, V - 1, 7, 3], device=DEV)
+    grads = []
+    for y in (bad, good):
+        x = z.clone().requires_grad_()
+        s = token_logprobs(x, y, top_k=5, entropy=True)
+        d, = torch.autograd.grad((s.entropy.sum(), s.top_logprobs.sum()), x, retain_graph=True)
+        full, = torch.autograd.grad(s.logprobs.sum(), x)
+        grads.append((s.entropy, s.top_ids, s.top_logprobs, d))
+        want = [y is bad] * 3 + [False]
+        assert s.logprobs.isnan().tolist() == want and full.isnan().all(1).tolist() == want and full.isnan().any(1).tolist() == want
+    assert all(torch.equal(a, b) and not a.isnan().any() for a, b in zip(*grads))
