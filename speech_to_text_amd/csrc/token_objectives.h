@@ -84,7 +84,9 @@ struct Out {
 constexpr int kGradWaves = 4, kGradVpt = 8;      // a gradient kernel's team, on a segment of at most 2048 vectors
 
 // ---------------------------------------------------------------------------------- which team takes a row
-constexpr int64_t kMaxBlocks = 2147483647;
+// Limits of a launch (2^31 blocks, 2^32 threads): a team of one or two waves a row at 2^24 rows is 2^31 threads, longer rows are
+// dealt; the gradients' kernels go in several launches.
+static_assert((int64_t)STTFE_MAX_ROWS * 64 * 2 < (1ll << 32), "a team a row");
 
 struct Plan {
     int team, segs, seg_len;

@@ -122,6 +122,7 @@ using namespace sttfe;
 extern "C" int sttfe_token_logprobs_workspace_bytes(int64_t rows, int vocab, int dtype, int top_k, size_t* bytes) {
     if (!bytes || rows < 0 || vocab < 1 || top_k < 0 || top_k > STTFE_MAX_TOP || top_k > vocab) return STTFE_E_INVALID_ARG;
     if (dtype != STTFE_DTYPE_F32 && dtype != STTFE_DTYPE_F16 && dtype != STTFE_DTYPE_BF16) return STTFE_E_INVALID_ARG;
+    if (rows > STTFE_MAX_ROWS || vocab > STTFE_MAX_VOCAB) return STTFE_E_UNSUPPORTED;
     const Plan plan = row_plan(vocab, dtype);
     *bytes = plan.segs == 1 ? 0 : (size_t)rows * plan.segs * (sizeof(float4) + sizeof(uint64_t) * (size_t)top_k);
     return STTFE_OK;
@@ -145,7 +146,6 @@ extern "C" int sttfe_token_logprobs(const void* logits, int dtype, int64_t outer
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = row_plan(vocab, dtype);
-    if (n > kMaxBlocks / plan.segs) return STTFE_E_UNSUPPORTED;
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     float4* parts = static_cast<float4*>(workspace);
     const int teams = dealt_teams(plan, n, kScoreAhead(top_k > 0));
@@ -173,7 +173,6 @@ extern "C" int sttfe_token_logprobs_grad(const void* logits, int dtype, int64_t 
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = grad_plan(vocab, dtype);
-    if (n > kMaxBlocks / plan.segs) return STTFE_E_UNSUPPORTED;
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     const ScoreGrad a{labels, ignore_index, (float)(kLog2e / (double)temperature), (float)(1.0 / (double)temperature), stats, g_logprobs,
                       g_entropy, top_k, top_ids, g_top};
@@ -194,6 +193,7 @@ static int check_distill(const int64_t* labels, const int64_t* ids, const float*
 extern "C" int sttfe_distill_workspace_bytes(int64_t rows, int vocab, int dtype, size_t* bytes) {
     if (!bytes || rows < 0 || vocab < 1) return STTFE_E_INVALID_ARG;
     if (dtype != STTFE_DTYPE_F32 && dtype != STTFE_DTYPE_F16 && dtype != STTFE_DTYPE_BF16) return STTFE_E_INVALID_ARG;
+    if (rows > STTFE_MAX_ROWS || vocab > STTFE_MAX_VOCAB) return STTFE_E_UNSUPPORTED;
     const Plan plan = row_plan(vocab, dtype);
     *bytes = plan.segs == 1 ? 0 : (size_t)rows * plan.segs * sizeof(float4) + (size_t)rows * 4 * sizeof(float);
     return STTFE_OK;
@@ -222,7 +222,6 @@ extern "C" int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, 
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = row_plan(vocab, dtype);
-    if (n > kMaxBlocks / plan.segs) return STTFE_E_UNSUPPORTED;
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     const Distill a = distill_args(labels, ignore_index, teacher_ids, teacher_logits, teacher_k, temperature, alpha);
     const Mode mode = distill_mode(a);
@@ -250,7 +249,6 @@ extern "C" int sttfe_distill_loss(const void* logits, int dtype, int64_t outer, 
             });
             if (grad) {
                 const Plan gp = grad_plan(vocab, dtype);
-                if (n > kMaxBlocks / gp.segs) return STTFE_E_UNSUPPORTED;
                 const Rows grows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, gp.segs, gp.seg_len};
                 STTFE_BY_DTYPE(dtype, Launch<T>::distill_grad(grows, a, mode, st, made, nullptr, nullptr, (unsigned)n, static_cast<T*>(grad), stream));
             }
@@ -278,7 +276,6 @@ extern "C" int sttfe_distill_grad(const void* logits, int dtype, int64_t outer, 
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
     (void)hipGetLastError();
     const Plan plan = grad_plan(vocab, dtype);
-    if (n > kMaxBlocks / plan.segs) return STTFE_E_UNSUPPORTED;
     const Rows rows{logits, (uint32_t)inner, stride_outer, stride_inner, vocab, plan.segs, plan.seg_len};
     const Distill a = distill_args(labels, ignore_index, teacher_ids, teacher_logits, teacher_k, temperature, alpha);
     {

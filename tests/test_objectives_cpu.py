@@ -216,3 +216,13 @@ def test_c_abi_refuses_unaligned_statistics_and_temperatures_out_of_range():
         for temp in (1e-7, 1e7, -1.0, float("nan"), float("inf")):
             assert call(temp=temp) == -1
     assert score(ws=odd) == -1 and distill(ws=odd) == -1
+
+
+def test_workspace_queries_know_the_limits():
+    L, n = _lib.lib(), ctypes.c_size_t()
+    for rows, V in ((2 ** 24 + 1, 11), (6, 2 ** 21 + 1), (6, 2 ** 31 - 1), (2 ** 62, 2 ** 31 - 1)):
+        assert L.sttfe_token_logprobs_workspace_bytes(rows, V, 0, 4, ctypes.byref(n)) == -5
+        assert L.sttfe_distill_workspace_bytes(rows, V, 0, ctypes.byref(n)) == -5
+    for dtype, e in ((0, 4), (1, 2), (2, 2)):
+        assert L.sttfe_token_logprobs_workspace_bytes(2 ** 24, 2 ** 21, dtype, 64, ctypes.byref(n)) == 0
+        assert n.value >= 2 ** 24 * (2 ** 21 * e // (2 ** 17)) * (16 + 8 * 64)

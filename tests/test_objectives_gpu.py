@@ -889,3 +889,30 @@ def test_entropy_and_alternatives_do_not_depend_on_the_label(V):
         want = [y is bad] * 3 + [False]
         assert s.logprobs.isnan().tolist() == want and full.isnan().all(1).tolist() == want and full.isnan().any(1).tolist() == want
     assert all(torch.equal(a, b) and not a.isnan().any() for a, b in zip(*grads))
+
+
+def test_as_many_rows_as_a_call_takes():
+    """2^24 rows, the most a call takes: 2^32 threads for the gradients are one too many for a launch.  Rows repeat, so a row's
+    result is known; the first, the last and those around the launches' border are looked at, and all by equality."""
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    n, V, period = 2 ** 24, 5, 64
+    z = randn((period, V), torch.bfloat16, 1)
+    y = torch.randint(0, V, (period,), generator=torch.Generator().manual_seed(2))
+    y[5] = -100
+    ids, t = teacher_rows(period, V, 2, 3)
+    lp, _, _, _ = O.token_logprobs(np64(z), y.numpy())
+    want_s, size_s = O.token_logprobs_grad(np64(z), y.numpy(), np.ones(period))
+    loss, want_d, size_d = O.distillation(np64(z), y.numpy(), ids.numpy(), t.numpy(), 3.0, 0.5)
+    x = z.to(DEV).repeat(n // period, 1).requires_grad_()
+    yy, ii, tt = (v.to(DEV).repeat(n // period, *([1] * (v.dim() - 1))) for v in (y, ids, t))
+    s = token_logprobs(x, yy)
+    same(np64(s.logprobs[-period:]), lp, (n_add(V) + 70 + 4 * np.abs(lp)) * U, "logprobs")
+    d, = torch.autograd.grad(s.logprobs.sum(), x)
+    check_grad(d[:period], want_s, size_s, torch.bfloat16, V)
+    assert bool((d.view(-1, period, V) == d[:period]).all())
+    each = distillation_loss(x, yy, ii, tt, temperature=3.0, reduction="none")
+    d, = torch.autograd.grad(each, x, torch.ones_like(each))
+    check_grad(d[:period], want_d, size_d, torch.bfloat16, V)
+    assert bool((d.view(-1, period, V) == d[:period]).all()) and bool((each.view(-1, period) == each[:period]).all())
+    with pytest.raises(Exception, match="unsupported|not supported|failed"):
+        token_logprobs(x.detach()[:1].expand(n + 1, V), top_k=1)
