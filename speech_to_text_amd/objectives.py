@@ -25,6 +25,7 @@ import ctypes
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -88,6 +89,15 @@ def _whole(t: torch.Tensor, shape, device, what: str, name: str) -> torch.Tensor
 def _on_gpu(logits: torch.Tensor, what: str):
     if logits.device.type != "cuda":
         raise _lib.SttfeError(f"{what}: logits are on {logits.device}: there is no CPU path")
+
+
+def _no_tangent(what: str, *tensors: torch.Tensor):
+    """Forward-mode derivatives: the kernels would drop the tangent of a dual tensor without a word."""
+    if getattr(forward_ad, "_current_level", 0) < 0:             # no dual level is open (looking at a tensor takes 0.7 us)
+        return
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what}: a tensor carries a forward-mode tangent; there are reverse-mode derivatives only")
 
 
 def _temperature(temperature: float, what: str) -> float:
@@ -156,6 +166,7 @@ class _TokenLogprobs(torch.autograd.Function):
         logits, labels, ids, stats = ctx.saved_tensors
         if g_logprobs is None and g_entropy is None and g_top is None:
             return (None,) * 7
+        _no_tangent("token_logprobs backward", *(t for t in (g_logprobs, g_entropy, g_top) if t is not None))
         top_k, temperature, ignore_index = ctx.args
         rows = _rows(logits, "token_logprobs")
         g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_logprobs, g_entropy, g_top)]
@@ -188,6 +199,7 @@ def token_logprobs(logits: torch.Tensor, labels: Optional[torch.Tensor] = None, 
     temperature = _temperature(temperature, what)
     if labels is not None:
         labels = _whole(labels, logits.shape[:-1], logits.device, what, "labels")
+    _no_tangent(what, logits)
     _on_gpu(logits, what)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenScores(*_TokenLogprobs.apply(logits, rows, labels, top_k, bool(entropy), temperature, int(ignore_index)))
@@ -214,6 +226,7 @@ def _distill_args(what, logits, labels, teacher_ids, teacher_logits, temperature
         raise ValueError(f"{what}: teacher_logits is a floating tensor of the shape and on the device of teacher_ids")
     if torch.is_grad_enabled() and t.requires_grad:
         raise ValueError(f"{what}: the teacher has no gradient here; detach() its logits")
+    _no_tangent(what, logits, t)
     if reduction == "none" and weight != 1.0:
         raise ValueError(f"{what}: weight belongs to a reduced loss; weight the positions' losses themselves")
     _on_gpu(logits, what)
@@ -263,6 +276,7 @@ class _Distillation(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, labels, ids, teacher, stats, factor = ctx.saved_tensors
+        _no_tangent("distillation_loss backward", g)
         g = g.to(torch.float32).contiguous()
         grad, ctx.grad = ctx.grad, None                 # handed out once: a second pass over a kept graph computes its own
         if grad is not None:
@@ -309,8 +323,11 @@ def distillation_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, teach
     that are captured into a graph or drive the model's backward themselves (``logits.backward(grad)``)."""
     if reduction == "none":
         raise ValueError("distillation_loss_and_grad: reduction is 'mean' or 'sum'")
-    logits = logits.detach()
-    args = _distill_args("distillation_loss_and_grad", logits, labels, teacher_ids, teacher_logits, temperature, alpha, ignore_index,
+    what = "distillation_loss_and_grad"
+    if torch.is_tensor(logits):
+        _no_tangent(what, logits)                    # detach() would drop it
+        logits = logits.detach()
+    args = _distill_args(what, logits, labels, teacher_ids, teacher_logits, temperature, alpha, ignore_index,
                          weight, reduction)
     loss, _, _, grad = _distill_forward(logits, args, False, True)
     return loss, grad

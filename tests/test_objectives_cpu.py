@@ -226,3 +226,19 @@ def test_workspace_queries_know_the_limits():
     for dtype, e in ((0, 4), (1, 2), (2, 2)):
         assert L.sttfe_token_logprobs_workspace_bytes(2 ** 24, 2 ** 21, dtype, 64, ctypes.byref(n)) == 0
         assert n.value >= 2 ** 24 * (2 ** 21 * e // (2 ** 17)) * (16 + 8 * 64)
+
+
+@pytest.mark.parametrize("call", [
+    lambda z, t: token_logprobs(z, Y, entropy=True),
+    lambda z, t: distillation_loss(z, Y, IDS, t),
+    lambda z, t: distillation_loss(Z, Y, IDS, t + 0 * z[..., :4]),
+    lambda z, t: distillation_loss_and_grad(z, Y, IDS, t),
+])
+def test_forward_mode_tangents_are_refused(call):
+    """A dual tensor does not require a gradient: its tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode tangent"):
+            call(forward_ad.make_dual(Z, torch.ones_like(Z)), T)
+        with pytest.raises(_lib.SttfeError, match="no CPU path"):
+            call(Z, T)

@@ -916,3 +916,16 @@ def test_as_many_rows_as_a_call_takes():
     assert bool((d.view(-1, period, V) == d[:period]).all()) and bool((each.view(-1, period) == each[:period]).all())
     with pytest.raises(Exception, match="unsupported|not supported|failed"):
         token_logprobs(x.detach()[:1].expand(n + 1, V), top_k=1)
+
+
+def test_forward_mode_tangent_of_an_upstream_gradient_is_refused():
+    from torch.autograd import forward_ad
+    from speech_to_text_amd import distillation_loss, token_logprobs
+    y, ids, t = torch.tensor([1, 2], device=DEV), torch.ones(2, 3, dtype=torch.long, device=DEV), torch.zeros(2, 3, device=DEV)
+    for f in (lambda x: token_logprobs(x, y).logprobs.sum(), lambda x: distillation_loss(x, y, ids, t)):
+        x = randn((2, 50), torch.float32, 1).to(DEV).requires_grad_()
+        loss = f(x)
+        with forward_ad.dual_level():
+            up = forward_ad.make_dual(torch.ones((), device=DEV), torch.ones((), device=DEV))
+            with pytest.raises(ValueError, match="forward-mode tangent"):
+                torch.autograd.grad(loss, x, up)
