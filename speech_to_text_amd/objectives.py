@@ -22,7 +22,7 @@ Results are float32 and on the logits' GPU; gradients have the logits' type.  Th
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple, Optional, Tuple
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch.autograd import forward_ad
@@ -317,17 +317,30 @@ def distillation_loss(logits: torch.Tensor, labels: torch.Tensor, teacher_ids: t
 
 def distillation_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, teacher_ids: torch.Tensor,
                                teacher_logits: torch.Tensor, *, temperature: float = 1.0, alpha: float = 0.5,
-                               ignore_index: int = -100, weight: float = 1.0,
-                               reduction: str = "mean") -> Tuple[torch.Tensor, torch.Tensor]:
+                               ignore_index: int = -100, weight: float = 1.0, reduction: str = "mean",
+                               grad_scale: Union[None, float, torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``distillation_loss`` ("mean" or "sum") and the gradient of the logits in one call without autograd, for training steps
-    that are captured into a graph or drive the model's backward themselves (``logits.backward(grad)``)."""
-    if reduction == "none":
-        raise ValueError("distillation_loss_and_grad: reduction is 'mean' or 'sum'")
+    that are captured into a graph or drive the model's backward themselves (``logits.backward(grad)``).
+
+    ``grad_scale`` multiplies the gradient, not the loss, before the gradient is rounded to the logits' type: a number, or a
+    float32 tensor of one element on the logits' GPU that the kernels read when they run.  float16 logits need a loss scale
+    here: the gradient's elements are p / positions, and what is below 3e-8 becomes 0, which no later scale brings back.
+    With it the logits are read a second time for the gradient."""
     what = "distillation_loss_and_grad"
+    if reduction == "none":
+        raise ValueError(f"{what}: reduction is 'mean' or 'sum'")
+    if torch.is_tensor(grad_scale) and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1
+                                        or not torch.is_tensor(logits) or grad_scale.device != logits.device):
+        raise ValueError(f"{what}: grad_scale is a number or a float32 tensor of one element on the device of the logits")
     if torch.is_tensor(logits):
         _no_tangent(what, logits)                    # detach() would drop it
         logits = logits.detach()
     args = _distill_args(what, logits, labels, teacher_ids, teacher_logits, temperature, alpha, ignore_index,
                          weight, reduction)
-    loss, _, _, grad = _distill_forward(logits, args, False, True)
-    return loss, grad
+    if grad_scale is None:
+        loss, _, _, grad = _distill_forward(logits, args, False, True)
+        return loss, grad
+    if not torch.is_tensor(grad_scale):
+        grad_scale = torch.full((), float(grad_scale), dtype=torch.float32, device=logits.device)
+    loss, factor, stats, _ = _distill_forward(logits, args, True, False)
+    return loss, _distill_backward(logits, args, stats, factor, grad_scale, None)

@@ -242,3 +242,10 @@ def test_forward_mode_tangents_are_refused(call):
             call(forward_ad.make_dual(Z, torch.ones_like(Z)), T)
         with pytest.raises(_lib.SttfeError, match="no CPU path"):
             call(Z, T)
+
+
+@pytest.mark.parametrize("scale", [torch.ones(2), torch.ones((), dtype=torch.float64), torch.ones((), dtype=torch.int64),
+                                   torch.ones((), device="meta")])
+def test_refused_scales_of_a_gradient(scale):
+    with pytest.raises(ValueError, match="grad_scale"):
+        distillation_loss_and_grad(Z, Y, IDS, T, grad_scale=scale)

@@ -929,3 +929,48 @@ def test_forward_mode_tangent_of_an_upstream_gradient_is_refused():
             up = forward_ad.make_dual(torch.ones((), device=DEV), torch.ones((), device=DEV))
             with pytest.raises(ValueError, match="forward-mode tangent"):
                 torch.autograd.grad(loss, x, up)
+
+
+@pytest.mark.parametrize("V", [2003, 10007, 140001])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_scaled_gradients(dtype, V):
+    """A loss scale is applied before the gradient is rounded: a float16 gradient of a mean keeps what it would lose (2^-25 is the
+    largest value that rounds to 0), every type has the oracle's gradient times the scale, the loss has no scale in it; numbers,
+    tensors, and a captured call whose scale changes between replays."""
+    from speech_to_text_amd import distillation_loss_and_grad
+    rows = 300 if V < 100000 else 40
+    z = randn((rows, V), TYPES[dtype], V, scale=2.0)
+    y = torch.randint(0, V, (rows,), generator=torch.Generator().manual_seed(V))
+    y[3] = -100
+    ids, teacher = teacher_rows(rows, V, 4, V)
+    some = [0, 1, 2, 3, 7, rows - 1]
+    _, grad, size = O.distillation(np64(z[some]), y.numpy()[some], ids.numpy()[some], teacher.numpy()[some], 2.0, 0.5)
+    f = 0.5 / (rows - 1)
+    x, args = z.to(DEV), (y.to(DEV), ids.to(DEV), teacher.to(DEV))
+    kw = dict(temperature=2.0, weight=0.5)
+    loss, plain = distillation_loss_and_grad(x, *args, **kw)
+    for scale in (2.0 ** 14, torch.full((1,), 2.0 ** 14, device=DEV), 3.0):
+        f_s = f * float(scale)
+        same_loss, g = distillation_loss_and_grad(x, *args, grad_scale=scale, **kw)
+        assert abs(float(same_loss) - float(loss)) <= 2 * (n_add(V) + 400) * 20 * U * abs(float(loss))
+        check_grad(g[some], grad * f_s, size * f_s, TYPES[dtype], V)
+        assert bool((g[3] == 0).all())
+    if dtype == "fp16":
+        lost = (np.abs(grad * f) < 2.0 ** -25) & (np.abs(grad * f) * 2.0 ** 14 > 2.0 ** -20)
+        scaled = distillation_loss_and_grad(x, *args, grad_scale=2.0 ** 14, **kw)[1]
+        assert lost.any() and (np64(plain[some])[lost] == 0).all() and (np64(scaled[some])[lost] != 0).all()
+    scale = torch.ones((), device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        distillation_loss_and_grad(x, *args, grad_scale=scale, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = distillation_loss_and_grad(x, *args, grad_scale=scale, **kw)
+    for k in (1.0, 64.0, 2.0 ** 14):
+        scale.fill_(k)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = distillation_loss_and_grad(x, *args, grad_scale=k, **kw)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
