@@ -356,7 +356,8 @@ int sttfe_distill_workspace_bytes(int64_t rows, int vocab, int dtype, size_t* by
  * q = softmax(teacher_logits / temperature) over the row's kept entries, p^t = softmax(logits / temperature),
  * p = softmax(logits).
  * teacher_ids / teacher_logits : device int64 / float32 [rows][teacher_k], teacher_k in [1, STTFE_MAX_TOP]; entries with a
- *                negative id are not kept, a row without any (or with only -inf logits) has no teacher term; the same id
+ *                negative id are not kept, a row without any (or with only -inf logits) has no teacher term (at alpha 1
+ *                it has none at all: loss and gradient are 0, whatever its logits are); the same id
  *                twice counts with both weights; an id >= vocab makes the row's loss and gradient NaN.
  * reduction    : NONE: losses only.  SUM / MEAN: factor[0] = weight (SUM) or weight / (number of rows whose label is not
  *                ignore_index; 1 if there is none) (MEAN), total[0] = factor[0] * (sum of the losses); device float32.

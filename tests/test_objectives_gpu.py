@@ -974,3 +974,29 @@ def test_scaled_gradients(dtype, V):
         torch.cuda.synchronize()
         want = distillation_loss_and_grad(x, *args, grad_scale=k, **kw)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("V", [1, 2, 300, 10007, 140001])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_rows_without_a_term_are_zero_whatever_they_hold(dtype, V):
+    """alpha 1 and no kept entry (no ids, or teacher logits of -inf): loss and gradient are 0, also of a row that has no softmax."""
+    from speech_to_text_amd import distillation_loss, distillation_loss_and_grad
+    z = randn((10, V), TYPES[dtype], V)
+    z[0], z[5] = -np.inf, -np.inf
+    z[1, V // 2] = z[6, V // 2] = np.nan
+    z[2, V - 1] = z[7, V - 1] = np.inf
+    z[3] = torch.finfo(TYPES[dtype]).min
+    y = torch.randint(0, V, (10,), generator=torch.Generator().manual_seed(V)).to(DEV)
+    ids = torch.full((10, 3), -1, device=DEV)
+    ids[4:9] = 0
+    t = torch.full((10, 3), -np.inf, device=DEV)
+    ids[9], t[9] = 0, 0.0                         # a sound row with a term
+    x = z.to(DEV).requires_grad_()
+    for tau in (1.0, 2.0):
+        each = distillation_loss(x, y, ids, t, temperature=tau, alpha=1.0, reduction="none")
+        d, = torch.autograd.grad(each, x, torch.ones(10, device=DEV))
+        s, = torch.autograd.grad(distillation_loss(x, y, ids, t, temperature=tau, alpha=1.0, reduction="sum"), x)
+        total, m = distillation_loss_and_grad(x, y, ids, t, temperature=tau, alpha=1.0, reduction="sum")
+        assert bool((each[:9] == 0).all()) and bool(total == each[9])
+        for g in (d, s, m):
+            assert bool((g[:9] == 0).all()) and not bool(g[9].isnan().any()) and (V == 1 or bool((g[9] != 0).any()))
