@@ -9,12 +9,12 @@ namespace sttfe {
 
 constexpr int kMaxWaves = 8, kMaxVpt = 16;       // the largest team: waves, and 16-byte vectors a thread holds
 // Whether a team that walks through rows loads the next one ahead. With alternatives to find it does not: the registers are worth
-// more as a second team on the CU, whose work fills the first one's exchanges (10240 x 50021 bf16, 16 alternatives: 0.37 ms
-// ahead, 0.32 ms two teams; without alternatives 0.24 ms against 0.33 ms).
+// more as a second team on the CU, whose work fills the first one's exchanges (10240 x 50021 bf16, 16 alternatives: 0.35 ms
+// ahead, 0.28 ms two teams; without alternatives 0.18 ms ahead, 0.19 ms two teams, with the entropy 0.20 against 0.21).
 constexpr bool kScoreAhead(bool top) { return !top; }
 constexpr bool kDistillAhead = true;
 constexpr int kWavesPerSimd(int vpt, bool ahead) { return vpt >= 16 && ahead ? 2 : 4; }
-// Alternatives of short rows: more waves in fewer registers (100000 x 2000 bf16, 16 alternatives: 0.20 ms with 4, 0.16 with 6).
+// Alternatives of short rows: more waves in fewer registers (100000 x 2000 bf16, 16 alternatives: 0.19 ms with 4, 0.15 with 6).
 constexpr int kScoreWaves(int waves, int vpt, bool top) { return top && waves == 1 ? 6 : kWavesPerSimd(vpt, kScoreAhead(top)); }
 constexpr int kGroups = 256;                     // groups of elements whose maxima bound the alternatives
 constexpr int kMaxSegs = 64;                     // segments of a row: one lane each when they are joined

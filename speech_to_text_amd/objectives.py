@@ -305,7 +305,8 @@ def distillation_loss(logits: torch.Tensor, labels: torch.Tensor, teacher_ids: t
     ``reduction``: "mean" over the positions whose label is not ``ignore_index`` (0 if there is none), "sum", or "none"
     (float32, shape of the labels).  ``weight`` multiplies the reduced loss (gradient accumulation: 1 / steps).
 
-    The gradient with respect to the logits has their type.  A label or id outside the vocabulary makes its position's loss
+    The gradient with respect to the logits has their type.  A reduced bfloat16 loss rounds it once for an upstream gradient of
+    1 and again for another one: ``weight`` rather than a factor on the loss keeps it at one.  A label or id outside the vocabulary makes its position's loss
     and gradient NaN.
     """
     args = _distill_args("distillation_loss", logits, labels, teacher_ids, teacher_logits, temperature, alpha, ignore_index, weight,
