@@ -334,7 +334,7 @@ def distillation_loss_and_grad(logits: torch.Tensor, labels: torch.Tensor, teach
                                         or not torch.is_tensor(logits) or grad_scale.device != logits.device):
         raise ValueError(f"{what}: grad_scale is a number or a float32 tensor of one element on the device of the logits")
     if torch.is_tensor(logits):
-        _no_tangent(what, logits)                    # detach() would drop it
+        _no_tangent(what, logits, *((grad_scale,) if torch.is_tensor(grad_scale) else ()))       # detach() would drop it
         logits = logits.detach()
     args = _distill_args(what, logits, labels, teacher_ids, teacher_logits, temperature, alpha, ignore_index,
                          weight, reduction)

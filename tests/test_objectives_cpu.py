@@ -249,3 +249,13 @@ def test_forward_mode_tangents_are_refused(call):
 def test_refused_scales_of_a_gradient(scale):
     with pytest.raises(ValueError, match="grad_scale"):
         distillation_loss_and_grad(Z, Y, IDS, T, grad_scale=scale)
+
+
+def test_forward_mode_tangent_of_a_scale_is_refused():
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        scale = forward_ad.make_dual(torch.ones(()), torch.ones(()))
+        with pytest.raises(ValueError, match="forward-mode tangent"):
+            distillation_loss_and_grad(Z, Y, IDS, T, grad_scale=scale)
+        with pytest.raises(_lib.SttfeError, match="no CPU path"):
+            distillation_loss_and_grad(Z, Y, IDS, T, grad_scale=torch.ones(()))
